@@ -64,16 +64,16 @@ __device__ __forceinline__ float nvfp4_silu(float x) {
   return __fdiv_rn(x, __fadd_rn(1.0f, nvfp4_expf(-x)));
 }
 
-// The same value for |x| <= 87 without a branch: nvfp4_expf without its range checks (the
-// argument cannot leave the range in which the two power-of-two factors are normal), and the
-// division as the reciprocal-refinement sequence behind the compiler's IEEE division - reciprocal
-// estimate, one Newton step, quotient, exact remainder, correction - without its check for
-// extreme exponents, which cannot occur here: the divisor lies in [1, 2^126] and the quotient is
-// a normal number. nvfp4_silu's two range checks and the division's out-of-line special-case path
-// are branches around every one of the sixteen values of a block, which serialise their
-// dependency chains (measured: ~270 cycles per value in the GEMM epilogue); this form lets the
-// sixteen chains overlap. Bit-identical to nvfp4_silu on every FP16 input in range (tested
-// exhaustively).
+// The same value for |x| <= 87 without nvfp4_expf's range checks (the argument cannot leave the
+// range in which the two power-of-two factors are normal) and without a full division. The quotient
+// is Markstein's (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", IBM J. Res. Dev. 34(1), 1990): with y = RN(1/d) and q0 = RN(x y), the remainder
+// x - d q0 is exact in one fused multiply-add and q0 + remainder * y rounds to RN(x / d). Nothing
+// over- or underflows on the way: the divisor lies in [1, 2^126] and the quotient is a normal
+// number. Range checks are branches around every one of the sixteen values of a block, which
+// serialise their dependency chains (measured: ~270 cycles per value in the GEMM epilogue);
+// without them the chains overlap. Bit-identical to nvfp4_silu on every FP16 input in range
+// (tested exhaustively).
 __device__ __forceinline__ float nvfp4_silu_in_range(float x) {
   const float a = -x;
   const float t = __fmul_rn(a, 1.44269504088896341f);
@@ -94,11 +94,9 @@ __device__ __forceinline__ float nvfp4_silu_in_range(float x) {
   const float s1 = __uint_as_float(static_cast<uint32_t>(h1 + 127) << 23);
   const float s2 = __uint_as_float(static_cast<uint32_t>(h2 + 127) << 23);
   const float d = __fadd_rn(1.0f, __fmul_rn(__fmul_rn(p, s1), s2));
-  float r0;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(d));
-  const float r1 = __fmaf_rn(r0, __fmaf_rn(-d, r0, 1.0f), r0);
-  const float q0 = __fmul_rn(x, r1);
-  const float q = __fmaf_rn(r1, __fmaf_rn(-d, q0, x), q0);
+  const float y = __frcp_rn(d);
+  const float q0 = __fmul_rn(x, y);
+  const float q = __fmaf_rn(__fmaf_rn(-d, q0, x), y, q0);
   // x = -0: the zero remainder would turn the quotient into +0; silu(x) always has the sign of x
   return __uint_as_float((__float_as_uint(q) & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u));
 }
