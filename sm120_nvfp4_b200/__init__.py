@@ -12,8 +12,9 @@ include/b200_nvfp4.h on torch's current stream. torch is used for memory and str
 from __future__ import annotations
 
 from .ops import (HostGemm, autotune_gemm, autotune_grouped_gemm, clear_tuned_tiles, cute_gemm, cutlass_gemm,
-                  expert_moe, expert_moe_workspace_bytes, fused_moe, gemm, grouped_gemm, pack_weights,
-                  quantize_expert, router_topk, scale_a_elements, scale_b_elements, scale_k_padded, tuned_tile)
+                  expert_moe, expert_moe_workspace_bytes, fp8_gemm, fp8_grouped_gemm, fused_moe, gemm, grouped_gemm,
+                  pack_weights, quantize_expert, quantize_fp8, router_backward, router_balance_loss, router_topk,
+                  router_topk_balanced, scale_a_elements, scale_b_elements, scale_k_padded, tuned_tile)
 
 __all__ = [
     "expert_moe",
@@ -30,6 +31,14 @@ __all__ = [
     # not in the reference package: the callers either side of the routed layer
     "router_topk",
     "pack_weights",
+    # FP8 products with a scale per block of 128, and the quantiser of their activations
+    "fp8_gemm",
+    "fp8_grouped_gemm",
+    "quantize_fp8",
+    # balance loss of the router, per-expert counts, gradients
+    "router_balance_loss",
+    "router_topk_balanced",
+    "router_backward",
     # host-memory operands, copies overlapped with the arithmetic
     "HostGemm",
     # shape-keyed tile table

@@ -71,6 +71,13 @@ _SIGNATURES = {
     "b200_nvfp4_set_fused_gate_up": (ci, [ci]),
     "b200_nvfp4_silu_f16": (ci, [vp, vp, ci, vp]),
     "b200_nvfp4_set_wait_limit": (ci, [C.c_longlong, ci]),
+    "b200_nvfp4_fp8_gemm": (ci, [ci, ci, ci, vp, vp, vp, vp, vp, ci, vp]),
+    "b200_nvfp4_fp8_grouped_gemm": (ci, [vp] * 7 + [ci] * 6 + [vp]),
+    "b200_nvfp4_fp8_set_tile": (ci, [ci, ci]),
+    "b200_nvfp4_fp8_quantize_rows": (ci, [vp, vp, vp, ci, ci, ci, ci, vp]),
+    "b200_nvfp4_moe_balance_loss_workspace_bytes": (C.c_size_t, [ci, ci, ci]),
+    "b200_nvfp4_moe_balance_loss": (ci, [vp] * 6 + [ci] * 6 + [C.c_float, vp, C.c_size_t, vp]),
+    "b200_nvfp4_moe_router_backward": (ci, [vp] * 8 + [ci] * 6 + [vp]),
     "b200_nvfp4_launch_count": (C.c_longlong, []),
 }
 

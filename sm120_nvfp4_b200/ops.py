@@ -611,6 +611,298 @@ def pack_weights(weight: torch.Tensor, weight_scale: Optional[torch.Tensor] = No
     return (packed, scales, alpha) if global_scale else (packed, scales)
 
 
+# ------------------------------------------------------------------------------------------
+# FP8 products with one FP32 scale per 128 values of K. Not in the reference package: checkpoints that
+# are FP8 with 128 x 128 block scales, or the parts of a model for which four bits are too few.
+
+_FP8 = getattr(torch, "float8_e4m3fn", None)
+_FP8_OUT = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+_INPUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _launch(device: torch.device, function: str, *args) -> None:
+    """Calls a C-ABI function with torch's current stream of `device` as its last argument; the device is
+    switched only where it is not the current one."""
+    call = getattr(_lib.lib(), function)
+    if torch.cuda.current_device() == device.index:
+        status = call(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = call(*args, _stream(device))
+    if status:
+        raise RuntimeError(f"{function} failed: {_lib.status_string(status)}")
+
+
+def _is_fp8(t: torch.Tensor) -> bool:
+    return t.dtype == _FP8 or t.dtype == torch.uint8
+
+
+def _blocks_128(n: int) -> int:
+    return (n + 127) // 128
+
+
+def quantize_fp8(x: torch.Tensor, *, swiglu: bool = False, output: Optional[torch.Tensor] = None,
+                 output_scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows to FP8 with one scale per 128 values: x [rows, K] (FP16, BF16 or FP32) -> (float8_e4m3fn
+    [rows, K], float32 scales [rows, ceil(K/128)]), value = code * scale. scale = amax / 448 of the block
+    (amax at least 2^-60), codes rounded to nearest. K must be a multiple of 16.
+
+    swiglu=True: x is [rows, 2K], gate columns then up columns, and silu(gate) * up is quantised - the
+    step between the two products of an expert. A block with a NaN or an infinity gets a NaN or
+    infinite scale. Not differentiable.
+    """
+    _check(x.is_cuda and x.dim() == 2 and x.is_contiguous() and x.dtype in _INPUT,
+           "x must be a contiguous FP16, BF16 or FP32 CUDA matrix")
+    rows, k = x.shape
+    if swiglu:
+        _check(k % 2 == 0, "x must hold gate and up columns")
+        k //= 2
+    _check(k > 0 and k % 16 == 0, "K must be a positive multiple of 16")
+    _check(x.data_ptr() % 16 == 0, "x must be 16-byte aligned")
+    device = x.device
+    if output is None:
+        output = torch.empty((rows, k), dtype=_FP8, device=device)
+    else:
+        _check_cuda_contig(output, device, "output")
+        _check(_is_fp8(output) and tuple(output.shape) == (rows, k) and output.data_ptr() % 16 == 0,
+               "output must be 16-byte aligned float8_e4m3fn (or uint8) [rows, K]")
+    if output_scale is None:
+        output_scale = torch.empty((rows, _blocks_128(k)), dtype=torch.float32, device=device)
+    else:
+        _check_cuda_contig(output_scale, device, "output_scale")
+        _check(output_scale.dtype == torch.float32 and tuple(output_scale.shape) == (rows, _blocks_128(k)),
+               "output_scale must be float32 [rows, ceil(K/128)]")
+    if rows:
+        _launch(device, "b200_nvfp4_fp8_quantize_rows", output.data_ptr(), output_scale.data_ptr(), x.data_ptr(), rows, k,
+                _INPUT[x.dtype], int(swiglu))
+    return output, output_scale
+
+
+def _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output, names):
+    device = x.device
+    for t, name in zip((x, weight, x_scale, weight_scale), names):
+        _check_cuda_contig(t, device, name)
+    _check(_is_fp8(x) and _is_fp8(weight), f"{names[0]} and {names[1]} must be float8_e4m3fn (or raw uint8 codes)")
+    _check(x_scale.dtype == torch.float32 and weight_scale.dtype == torch.float32, "scales must be float32")
+    _check(x.dim() == 2 and x.size(1) == weight.size(-1), f"{names[0]} and {names[1]} must share K")
+    rows, k = x.shape
+    n = weight.size(-2)
+    _check(k > 0 and k % 16 == 0, "K must be a positive multiple of 16")
+    _check(n > 0 and n % 8 == 0, "N must be a positive multiple of 8")
+    kb = _blocks_128(k)
+    _check(tuple(x_scale.shape) == (rows, kb), f"{names[2]} must be [rows, ceil(K/128)]")
+    _check(tuple(weight_scale.shape) == (*weight.shape[:-2], _blocks_128(n), kb),
+           f"{names[3]} must hold one scale per 128 x 128 block of {names[1]}")
+    _check(x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0, f"{names[0]} and {names[1]} must be 16-byte aligned")
+    if output is None:
+        _check(out_dtype in _FP8_OUT, "out_dtype must be float16, bfloat16 or float32")
+        output = torch.empty((rows, n), dtype=out_dtype, device=device)
+    else:
+        _check_cuda_contig(output, device, "output")
+        _check(output.dtype in _FP8_OUT and tuple(output.shape) == (rows, n) and output.data_ptr() % 16 == 0,
+               "output must be a 16-byte aligned FP16, BF16 or FP32 matrix [rows, N]")
+        _check(out_dtype is None or out_dtype == output.dtype, "out_dtype does not match output")
+    return rows, n, k, output
+
+
+def fp8_gemm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, *,
+             out_dtype: Optional[torch.dtype] = None, output: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """FP8 product with block scales: a [M, K] times b [N, K] transposed, both float8_e4m3fn (or the raw
+    bytes), a_scale float32 [M, ceil(K/128)] (one per row and 128 values, as quantize_fp8 makes them),
+    b_scale float32 [ceil(N/128), ceil(K/128)] (one per 128 x 128 block, as FP8 checkpoints hold them).
+    FP32 sums, one rounding to out_dtype (FP16 by default, BF16 or FP32; that of `output` where given).
+    M may be 0; N % 8 == 0, K % 16 == 0.
+
+    Not differentiable. The gradient with respect to the input is the same product: quantize_fp8(grad)
+    times b.t().contiguous() with b_scale.t().contiguous().
+    """
+    _check(a.is_cuda, "a must be a CUDA tensor")
+    _check(b.dim() == 2, "b must be [N, K]")
+    if out_dtype is None and output is None:
+        out_dtype = torch.float16
+    m, n, k, out = _fp8_operands(a, b, a_scale, b_scale, out_dtype, output, ("a", "b", "a_scale", "b_scale"))
+    if m:
+        _launch(a.device, "b200_nvfp4_fp8_gemm", m, n, k, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
+                out.data_ptr(), _FP8_OUT[out.dtype])
+    return out
+
+
+def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tensor, cu_seqlens: torch.Tensor,
+                     x_scale: torch.Tensor, weight_scale: torch.Tensor, *, out_dtype: Optional[torch.dtype] = None,
+                     output: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The FP8 product per expert, one launch: rows [cu_seqlens[g], cu_seqlens[g] + seqlens[g]) of x
+    [rows, K] times weight[g] ([groups, N, K]) transposed; x_scale [rows, ceil(K/128)], weight_scale
+    [groups, ceil(N/128), ceil(K/128)]. seqlens int32 [groups] and cu_seqlens int32 [groups + 1] stay on
+    the device; the ranges must not overlap. Rows that belong to no group keep what `output` held (without
+    `output` they are undefined). groups <= 256; otherwise as fp8_gemm.
+    """
+    _check(x.is_cuda, "x must be a CUDA tensor")
+    _check(weight.dim() == 3, "weight must be [groups, N, K]")
+    if out_dtype is None and output is None:
+        out_dtype = torch.float16
+    rows, n, k, out = _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output,
+                                    ("x", "weight", "x_scale", "weight_scale"))
+    groups = weight.size(0)
+    _check(0 < groups <= 256, "number of groups must be in [1, 256]")
+    for t, name in ((seqlens, "seqlens"), (cu_seqlens, "cu_seqlens")):
+        _check_cuda_contig(t, x.device, name)
+        _check(t.dtype == torch.int32, "seqlens and cu_seqlens must be int32")
+    _check(seqlens.numel() == groups and cu_seqlens.numel() == groups + 1,
+           "seqlens / cu_seqlens lengths are inconsistent with the number of groups")
+    if rows:
+        _launch(x.device, "b200_nvfp4_fp8_grouped_gemm", out.data_ptr(), x.data_ptr(), weight.data_ptr(), seqlens.data_ptr(),
+                cu_seqlens.data_ptr(), x_scale.data_ptr(), weight_scale.data_ptr(), groups, rows, n, k, 0,
+                _FP8_OUT[out.dtype])
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# Training side of the router step: balance loss, per-expert counts and the gradient of the logits.
+
+_SCORING = {"sigmoid": 0, "softmax": 1}
+
+
+def _check_router(logits, topk_ids, cu_seqlens, scoring):
+    _check(logits.is_cuda and logits.dim() == 2 and logits.is_contiguous() and logits.dtype in _INPUT,
+           "logits must be a contiguous FP32, BF16 or FP16 CUDA tensor [num_tokens, num_experts]")
+    t, e = logits.shape
+    _check_cuda_contig(topk_ids, logits.device, "topk_ids")
+    _check(topk_ids.dtype == torch.int32 and topk_ids.dim() == 2 and topk_ids.size(0) == t,
+           "topk_ids must be int32 [num_tokens, num_topk]")
+    _check(0 < topk_ids.size(1) <= e <= 4096, "need 0 < num_topk <= num_experts <= 4096")
+    _check(scoring in _SCORING, "scoring must be 'sigmoid' or 'softmax'")
+    sequences = 1
+    if cu_seqlens is not None:
+        _check_cuda_contig(cu_seqlens, logits.device, "cu_seqlens")
+        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 2 <= cu_seqlens.numel() <= 65537,
+               "cu_seqlens must be int32 [num_sequences + 1] with at most 65536 sequences")
+        sequences = cu_seqlens.numel() - 1
+    return t, e, topk_ids.size(1), sequences
+
+
+def _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha):
+    t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
+    device = logits.device
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    counts = torch.empty((sequences, e), dtype=torch.int32, device=device)
+    slope = torch.empty((sequences, e), dtype=torch.float32, device=device)
+    need = _lib.lib().b200_nvfp4_moe_balance_loss_workspace_bytes(t, e, sequences)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _launch(device, "b200_nvfp4_moe_balance_loss", loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), logits.data_ptr(),
+            topk_ids.data_ptr(), _ptr(cu_seqlens), t, e, k, sequences, _INPUT[logits.dtype], _SCORING[scoring], float(alpha),
+            workspace.data_ptr(), need)
+    return loss, counts, slope
+
+
+def router_backward(logits: torch.Tensor, topk_ids: torch.Tensor, *, topk_weights: Optional[torch.Tensor] = None,
+                    grad_weights: Optional[torch.Tensor] = None, slope: Optional[torch.Tensor] = None,
+                    grad_loss: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                    scoring: str = "sigmoid") -> torch.Tensor:
+    """Gradient of the router's logits in one pass: through the weights of router_topk (topk_weights and
+    grad_weights float32 [T, k]), through the balance loss (slope from router_balance_loss, grad_loss a
+    float32 scalar on the device), or both. Returns a tensor of the logits' type and shape. What the
+    autograd forms call; takes part in CUDA-graph capture like any other call.
+
+    `scoring` is that of the loss; the weights are router_topk's (sigmoid). Slots with an id outside
+    [0, E) are empty; slots of a token that name the same expert add up.
+    """
+    t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
+    _check(grad_weights is not None or slope is not None, "grad_weights or slope must be given")
+    device = logits.device
+    if grad_weights is not None:
+        _check(topk_weights is not None, "grad_weights needs topk_weights")
+        for x, name in ((topk_weights, "topk_weights"), (grad_weights, "grad_weights")):
+            _check_cuda_contig(x, device, name)
+            _check(x.dtype == torch.float32 and x.shape == topk_ids.shape, "topk_weights and grad_weights must be float32 [T, k]")
+    if slope is not None:
+        _check(grad_loss is not None, "slope needs grad_loss")
+        _check_cuda_contig(slope, device, "slope")
+        _check(slope.dtype == torch.float32 and tuple(slope.shape) == (sequences, e),
+               "slope must be float32 [num_sequences, num_experts]")
+        _check(grad_loss.is_cuda and grad_loss.device == device and grad_loss.dtype == torch.float32 and grad_loss.numel() == 1,
+               "grad_loss must be one float32 on the device of the logits")
+    grad = torch.empty_like(logits)
+    if t:
+        _launch(device, "b200_nvfp4_moe_router_backward", grad.data_ptr(), logits.data_ptr(), topk_ids.data_ptr(),
+                _ptr(topk_weights), _ptr(grad_weights), _ptr(slope), _ptr(grad_loss) if slope is not None else None,
+                _ptr(cu_seqlens), t, e, k, sequences, _INPUT[logits.dtype], _SCORING[scoring])
+    return grad
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk_ids, cu_seqlens, scoring, alpha):
+        loss, counts, slope = _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha)
+        ctx.save_for_backward(logits, topk_ids, cu_seqlens, slope)
+        ctx.scoring = scoring
+        ctx.mark_non_differentiable(counts, slope)
+        return loss, counts, slope
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _counts, _slope):
+        logits, topk_ids, cu_seqlens, slope = ctx.saved_tensors
+        grad = router_backward(logits, topk_ids, slope=slope, grad_loss=grad_loss.contiguous(), cu_seqlens=cu_seqlens,
+                               scoring=ctx.scoring)
+        return grad, None, None, None, None
+
+
+class _TopkBalanced(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, num_topk, cu_seqlens, scoring, alpha):
+        ids, weights = router_topk(logits, num_topk)
+        loss, counts, slope = _balance_forward(logits, ids, cu_seqlens, scoring, alpha)
+        ctx.save_for_backward(logits, ids, weights, cu_seqlens, slope)
+        ctx.scoring = scoring
+        ctx.mark_non_differentiable(ids, counts)
+        ctx.set_materialize_grads(False)
+        return ids, weights, loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _ids, grad_weights, grad_loss, _counts):
+        logits, ids, weights, cu_seqlens, slope = ctx.saved_tensors
+        if grad_weights is None and grad_loss is None:
+            return None, None, None, None, None
+        grad = router_backward(logits, ids, topk_weights=weights,
+                               grad_weights=None if grad_weights is None else grad_weights.contiguous(),
+                               slope=None if grad_loss is None else slope,
+                               grad_loss=None if grad_loss is None else grad_loss.contiguous(),
+                               cu_seqlens=cu_seqlens, scoring=ctx.scoring)
+        return grad, None, None, None, None
+
+
+def router_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                        scoring: str = "sigmoid", alpha: float = 1.0
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Balance loss of a routing decision, with per-expert counts: logits [T, E] (FP32, BF16 or FP16),
+    topk_ids int32 [T, k], cu_seqlens int32 [S + 1] (packed sequences; None: one sequence) -> (loss float32
+    scalar, counts int32 [S, E], slope float32 [S, E]).
+
+    Per sequence alpha * sum_e f_e P_e with f_e = counts_e E / (k T_s) and P_e the mean of the token's
+    normalised scores (sigmoid scores over their sum, or softmax); the loss is the mean over sequences that
+    have a token. A token outside every sequence, or whose ids all lie outside [0, E), is masked. The
+    loss is differentiable with respect to the logits (counts are constants); slope is what
+    router_backward needs to do the same by hand.
+    """
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _BalanceLoss.apply(logits, topk_ids, cu_seqlens, scoring, alpha)
+    return _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha)
+
+
+def router_topk_balanced(logits: torch.Tensor, num_topk: int, *, cu_seqlens: Optional[torch.Tensor] = None,
+                         scoring: str = "sigmoid", alpha: float = 1.0
+                         ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """router_topk for a router in training: FP32 logits [T, E] -> (topk_ids, topk_weights, loss, counts),
+    ids and weights exactly router_topk's, loss and counts those of router_balance_loss. weights and loss
+    are differentiable with respect to the logits; the backward pass is one kernel for both.
+    """
+    _check(logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32 and logits.is_contiguous(),
+           "logits must be a contiguous float32 CUDA tensor [num_tokens, num_experts]")
+    _check(scoring in _SCORING, "scoring must be 'sigmoid' or 'softmax'")
+    return _TopkBalanced.apply(logits, num_topk, cu_seqlens, scoring, alpha)
+
+
 # ---------------------------------------------------------------------------------- tile table
 #
 # Not in the reference package (its RTX 5090 tuning is compiled in): times the tile shapes of the
