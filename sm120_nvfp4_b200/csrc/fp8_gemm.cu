@@ -107,7 +107,7 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
     cudaFuncAttributes attr;
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, fp8_pair_kernel);
     // the kernel moves registers between its warpgroups: it must have been launched with all of them
-    if (e == cudaSuccess && attr.numRegs * Cfg::kThreads < 56 * 128 + 224 * 256) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess && attr.numRegs * Cfg::kThreads < 72 * 128 + 216 * 256) e = cudaErrorInvalidConfiguration;
     attr_status[dev.device] = e;
     max_pairs[dev.device] = e == cudaSuccess ? resident_clusters(fp8_pair_kernel, dev, 2, Cfg::kThreads, kSmemBudget) : 0;
   });
@@ -123,6 +123,7 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
   p.tma_store = q.n >= (f32 ? 32 : 64) &&
                 encode_tmap_2d_out(&tmap_out, p.out, static_cast<uint64_t>(q.rows), static_cast<uint64_t>(q.n),
                                    static_cast<uint64_t>(q.n), f32, 32, f32 ? 32 : 64);
+  p.scales_by_16 = (q.k + kFp8BlockK - 1) / kFp8BlockK % 4 == 0 && aligned16(p.a_scale) && aligned16(p.b_scale);
   p.splits = 1;
   p.num_stages = Cfg::stages_for(q.groups);
   p.raster_m = 8;

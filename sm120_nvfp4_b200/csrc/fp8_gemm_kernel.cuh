@@ -31,7 +31,8 @@
 namespace b200 {
 
 constexpr int kFp8BlockK = 128;               // values of K per scale = bytes of K per stage row
-constexpr int kFp8ScaleSlots = 8;             // ring of scale vectors
+constexpr int kFp8Panel = 8;                  // blocks of K whose scales arrive together ...
+constexpr int kFp8Panels = 2;                 // ... and panels in shared memory
 
 enum Fp8Out { kOutF16 = 0, kOutF32 = 1, kOutBf16 = 2 };
 
@@ -47,6 +48,7 @@ struct Fp8Params {
   int out_type;               // Fp8Out
   int raster_m;
   int num_stages;
+  int scales_by_16;           // scale rows start on 16-byte boundaries: whole panels by 16-byte copies
   int splits;                 // skinny kernel: CTAs of a cluster over K
   int tma_store;
   int* error;
@@ -88,6 +90,31 @@ __device__ __forceinline__ void fp8_group_tables(const Fp8Params& p, int tile_ro
   __syncthreads();
 }
 
+// Starts the copies of one panel of scales into shared memory, [block][stride] floats: the scales of
+// `count` blocks of K from b0 on for ROWS rows, of which the first `valid` exist (the others become
+// zeros), and behind them those of TILES column tiles of B. Rows are kb floats apart in memory and of
+// any alignment, so the copies are 4 bytes each; eight neighbouring lanes take a row's eight blocks, which
+// is one sector (with a row per lane every copy was a sector of its own, and the eight blocks of a panel
+// fetched each of them again: the loader could not keep up with the MMAs).
+template <int ROWS, int TILES>
+__device__ __forceinline__ void fp8_load_scales(uint32_t dst, int stride, const float* a_scale, long long row, int valid, int kb,
+                                                int b0, int count, const float* b_scale, int tiles_left, int lane) {
+  const int j = lane & 7;
+  const bool block_in = j < count;
+  const float* src = a_scale + (row + (lane >> 3)) * kb + b0 + j;
+  const uint32_t to = dst + static_cast<uint32_t>(j * stride + (lane >> 3)) * 4;
+#pragma unroll 8
+  for (int r = 0; r < ROWS; r += 4) {
+    const bool in = r + (lane >> 3) < valid;
+    if (block_in) ptx::cp_async_4(to + 4 * r, in ? src + static_cast<long long>(r) * kb : a_scale, in);
+  }
+  const int tile = lane >> 3;
+  if (tile < TILES && block_in) {
+    const bool in = tile < tiles_left;
+    ptx::cp_async_4(dst + static_cast<uint32_t>(j * stride + ROWS + tile) * 4, in ? b_scale + static_cast<long long>(tile) * kb + b0 + j : b_scale, in);
+  }
+}
+
 // One output value, rounded once from FP32.
 __device__ __forceinline__ void fp8_store(void* out, int type, long long at, float v) {
   if (type == kOutF16) static_cast<__half*>(out)[at] = __float2half_rn(v);
@@ -113,10 +140,10 @@ struct Fp8SkinnyCfg {
   static constexpr int kXBytes = BN * kFp8BlockK;
   static constexpr int kStageBytes = kWBytes + kXBytes;
   static constexpr int kMaxStages = 12;
-  static constexpr int kSlotFloats = BN + 4;  // row scales of one block, then the scale of the weights' tile
+  static constexpr int kSlotFloats = BN + 4;  // row scales of one block, then the scale of the weights' tile (multiple of 4)
   static constexpr int kRedBytes = 128 * BN * 4;
   static constexpr int fixed_bytes(int groups, int splits) {
-    return 1024 + 512 + kFp8ScaleSlots * kSlotFloats * 4 + 3 * (groups + 1) * 4 + (splits > 1 ? kRedBytes : 0);
+    return 1024 + 512 + kFp8Panels * kFp8Panel * kSlotFloats * 4 + 3 * (groups + 1) * 4 + (splits > 1 ? kRedBytes : 0);
   }
   static constexpr int stages_for(int groups, int splits) {
     const int s = (kSmemBudget - fixed_bytes(groups, splits)) / kStageBytes;
@@ -147,12 +174,12 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   const uint32_t sum_full_u32 = empty_u32 + 8 * Cfg::kMaxStages;       // a block's sums are in tensor memory
   const uint32_t sum_empty_u32 = sum_full_u32 + 8 * Cfg::kBuffers;     // ... have been read
   const uint32_t sc_full_u32 = sum_empty_u32 + 8 * Cfg::kBuffers;      // a block's scales are in their slot
-  const uint32_t sc_empty_u32 = sc_full_u32 + 8 * kFp8ScaleSlots;
-  const uint32_t red_full_u32 = sc_empty_u32 + 8 * kFp8ScaleSlots;     // every CTA's part of this CTA's columns
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kMaxStages + 2 * Cfg::kBuffers + 2 * kFp8ScaleSlots + 1);
+  const uint32_t sc_empty_u32 = sc_full_u32 + 8 * kFp8Panels;
+  const uint32_t red_full_u32 = sc_empty_u32 + 8 * kFp8Panels;     // every CTA's part of this CTA's columns
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kMaxStages + 2 * Cfg::kBuffers + 2 * kFp8Panels + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
   float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);
-  int* s_cu_tiles = reinterpret_cast<int*>(slots + kFp8ScaleSlots * Cfg::kSlotFloats);
+  int* s_cu_tiles = reinterpret_cast<int*>(slots + kFp8Panels * kFp8Panel * Cfg::kSlotFloats);
   int* s_row0 = s_cu_tiles + (p.num_groups + 1);
   int* s_rows = s_row0 + (p.num_groups + 1);
 
@@ -173,7 +200,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       ptx::mbar_init(sum_full_u32 + 8 * lane, 1);
       ptx::mbar_init(sum_empty_u32 + 8 * lane, 4);
     }
-    if (lane < kFp8ScaleSlots) {
+    if (lane < kFp8Panels) {
       ptx::mbar_init(sc_full_u32 + 8 * lane, 32);
       ptx::mbar_init(sc_empty_u32 + 8 * lane, 4);
     }
@@ -225,9 +252,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     }
     __syncwarp();
   } else if (warp == kLoadS) {
-    // 4-byte asynchronous copies: the scales of one block are kb floats apart in memory. Rows behind
-    // the end are not read and become zeros.
-    int slot = 0;
+    int panel = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
@@ -235,20 +260,12 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       const int row = s_row0[t.g] + t.mt * BN;
       const int valid = min(BN, s_rows[t.g] - t.mt * BN);
       const float* sb = p.b_scale + (static_cast<long long>(t.g) * n_tiles + t.nt) * kb;
-      for (int b = b_begin; b < b_end; ++b) {
-        if (!ptx::mbar_wait(sc_empty_u32 + 8 * slot, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
-        const uint32_t dst = ptx::smem_u32(slots + slot * Cfg::kSlotFloats);
-#pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += 32) {
-          const int c = c0 + lane;
-          if (c < BN) {
-            const bool in = c < valid;
-            ptx::cp_async_4(dst + 4 * c, p.a_scale + static_cast<long long>(in ? row + c : row) * kb + b, in);
-          }
-        }
-        if (lane == 0) ptx::cp_async_4(dst + 4 * BN, sb + b, true);
-        ptx::cp_async_mbar_arrive(sc_full_u32 + 8 * slot);
-        if (++slot == kFp8ScaleSlots) { slot = 0; phase ^= 1; }
+      for (int b0 = b_begin; b0 < b_end; b0 += kFp8Panel) {
+        if (!ptx::mbar_wait(sc_empty_u32 + 8 * panel, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
+        fp8_load_scales<BN, 1>(ptx::smem_u32(slots + panel * kFp8Panel * Cfg::kSlotFloats), Cfg::kSlotFloats, p.a_scale, row, valid,
+                               kb, b0, b_end - b0, sb, 1, lane);
+        ptx::cp_async_mbar_arrive(sc_full_u32 + 8 * panel);
+        if (++panel == kFp8Panels) { panel = 0; phase ^= 1; }
       }
     }
     ptx::cp_async_wait_all();
@@ -284,8 +301,8 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     const int q = warp & 3;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
     constexpr int kChunk = BN < 32 ? BN : 32;
-    int buf = 0, slot = 0;
-    uint32_t buf_phase = 0, slot_phase = 0;
+    int buf = 0, panel = 0;
+    uint32_t buf_phase = 0, panel_phase = 0;
     bool ok = true;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
       const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
@@ -294,10 +311,11 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 #pragma unroll
       for (int c = 0; c < BN; ++c) acc[c] = 0.0f;
       for (int b = b_begin; b < b_end; ++b) {
-        if (!ptx::mbar_wait(sc_full_u32 + 8 * slot, slot_phase, abort_flag, kWaitSlots, p.wait_limit) ||
+        const int in_panel = (b - b_begin) & (kFp8Panel - 1);
+        if ((in_panel == 0 && !ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) ||
             !ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
         ptx::tc_fence_after_sync();
-        const float* sc = slots + slot * Cfg::kSlotFloats;
+        const float* sc = slots + (panel * kFp8Panel + in_panel) * Cfg::kSlotFloats;
         const float sb = sc[BN];
 #pragma unroll
         for (int c0 = 0; c0 < BN; c0 += kChunk) {
@@ -315,12 +333,13 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         }
         ptx::tc_fence_before_sync();
         __syncwarp();
+        const bool panel_done = in_panel == kFp8Panel - 1 || b + 1 == b_end;
         if (lane == 0) {
           ptx::mbar_arrive(sum_empty_u32 + 8 * buf);
-          ptx::mbar_arrive(sc_empty_u32 + 8 * slot);
+          if (panel_done) ptx::mbar_arrive(sc_empty_u32 + 8 * panel);
         }
         if (++buf == Cfg::kBuffers) { buf = 0; buf_phase ^= 1; }
-        if (++slot == kFp8ScaleSlots) { slot = 0; slot_phase ^= 1; }
+        if (panel_done && ++panel == kFp8Panels) { panel = 0; panel_phase ^= 1; }
       }
       if (!ok) break;
       const int tile_row = q * 32 + lane;
@@ -396,7 +415,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 // MMAs read both halves, and each CTA's tensor memory receives 128 rows x 256 columns of a block's
 // sums. Two such buffers fill the 512 columns of tensor memory. 128 accumulators per thread in eight
 // promotion warps need more registers than an even share (65536 / 384 = 168): the other four warps
-// give theirs up (56 + 2 x 224 = 504 = 3 x 168 per three warpgroups' lanes).
+// give theirs up (72 + 2 x 216 = 504 = 3 x 168).
 struct Fp8PairCfg {
   static constexpr int kThreads = 384;
   static constexpr int kBuffers = 2;
@@ -404,10 +423,14 @@ struct Fp8PairCfg {
   static constexpr int kBBytes = 128 * kFp8BlockK;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kMaxStages = 6;
-  static constexpr int kSlotFloats = 128 + 4;                    // scales of the CTA's rows, of two column tiles
+  // Scales arrive in panels of four blocks of K, [row][block]: a promotion thread takes its row's four
+  // with one 16-byte read. Two more rows hold those of the tile's two 128-column tiles of B.
+  static constexpr int kPanel = 4;
+  static constexpr int kPanels = 4;
+  static constexpr int kPanelFloats = (128 + 2) * kPanel;
   static constexpr int kStagingBytes = 8 * 32 * 128;
   static constexpr int fixed_bytes(int groups) {
-    return 1024 + 512 + kFp8ScaleSlots * kSlotFloats * 4 + 3 * (groups + 1) * 4 + kStagingBytes;
+    return 1024 + 512 + kPanels * kPanelFloats * 4 + 3 * (groups + 1) * 4 + kStagingBytes;
   }
   static constexpr int stages_for(int groups) {
     const int s = (kSmemBudget - fixed_bytes(groups)) / kStageBytes;
@@ -435,11 +458,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   const uint32_t sum_full_u32 = empty_u32 + 8 * Cfg::kMaxStages;
   const uint32_t sum_empty_u32 = sum_full_u32 + 8 * Cfg::kBuffers;
   const uint32_t sc_full_u32 = sum_empty_u32 + 8 * Cfg::kBuffers;
-  const uint32_t sc_empty_u32 = sc_full_u32 + 8 * kFp8ScaleSlots;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kMaxStages + 2 * Cfg::kBuffers + 2 * kFp8ScaleSlots);
+  const uint32_t sc_empty_u32 = sc_full_u32 + 8 * Cfg::kPanels;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kMaxStages + 2 * Cfg::kBuffers + 2 * Cfg::kPanels);
   int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
   float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);
-  int* s_cu_tiles = reinterpret_cast<int*>(slots + kFp8ScaleSlots * Cfg::kSlotFloats);
+  int* s_cu_tiles = reinterpret_cast<int*>(slots + Cfg::kPanels * Cfg::kPanelFloats);
   int* s_row0 = s_cu_tiles + (p.num_groups + 1);
   int* s_rows = s_row0 + (p.num_groups + 1);
 
@@ -459,9 +482,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     if (lane < Cfg::kBuffers) {
       ptx::mbar_init(sum_full_u32 + 8 * lane, 1);
-      ptx::mbar_init(sum_empty_u32 + 8 * lane, 16);
+      ptx::mbar_init(sum_empty_u32 + 8 * lane, 16);    // eight promotion warps of each CTA
     }
-    if (lane < kFp8ScaleSlots) {
+    if (lane < Cfg::kPanels) {
       ptx::mbar_init(sc_full_u32 + 8 * lane, 32);
       ptx::mbar_init(sc_empty_u32 + 8 * lane, 8);
     }
@@ -490,7 +513,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
   // (each share is set where its code begins: after a join the compiler would hold both to the smaller)
   if (warp < kFirstPromoter) {
-  ptx::setmaxnreg_dec<56>();
+  ptx::setmaxnreg_dec<72>();
   if (warp == kLoadA || warp == kLoadB) {
     const bool is_a = warp == kLoadA;
     const CUtensorMap* tmap = is_a ? &tmap_a : &tmap_b;
@@ -514,7 +537,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     __syncwarp();
   } else if (warp == kLoadS) {
-    int slot = 0;
+    int panel = 0;
     uint32_t phase = 0;
     bool ok = true;
     const int nb = (p.n + 127) / 128;
@@ -523,21 +546,31 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const int row = s_row0[t.g] + t.mt * 256 + cta * 128;
       const int valid = min(128, s_rows[t.g] - t.mt * 256 - cta * 128);     // may be <= 0 in the second CTA
       const float* sb = p.b_scale + (static_cast<long long>(t.g) * nb + 2 * t.nt) * kb;
-      for (int b = 0; b < kb; ++b) {
-        if (!ptx::mbar_wait(sc_empty_u32 + 8 * slot, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
-        const uint32_t dst = ptx::smem_u32(slots + slot * Cfg::kSlotFloats);
+      for (int b0 = 0; b0 < kb; b0 += Cfg::kPanel) {
+        if (!ptx::mbar_wait(sc_empty_u32 + 8 * panel, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
+        const uint32_t dst = ptx::smem_u32(slots + panel * Cfg::kPanelFloats);
+        if (p.scales_by_16) {
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          const int c = c0 + lane;
-          const bool in = c < valid;
-          ptx::cp_async_4(dst + 4 * c, p.a_scale + (in ? static_cast<long long>(row + c) * kb + b : 0), in);
-        }
-        if (lane < 2) {
+          for (int c0 = 0; c0 < 128; c0 += 32) {
+            const int c = c0 + lane;
+            const bool in = c < valid;
+            ptx::cp_async_16(dst + 16 * c, in ? p.a_scale + static_cast<long long>(row + c) * kb + b0 : p.a_scale, in);
+          }
           const bool in = 2 * t.nt + lane < nb;
-          ptx::cp_async_4(dst + 4 * (128 + lane), sb + (in ? static_cast<long long>(lane) * kb : 0) + b, in);
+          if (lane < 2) ptx::cp_async_16(dst + 16 * (128 + lane), in ? sb + static_cast<long long>(lane) * kb + b0 : p.b_scale, in);
+        } else {
+          const int j = lane & 3, r0 = lane >> 2;
+          const bool block_in = b0 + j < kb;
+#pragma unroll 4
+          for (int r = r0; r < 128; r += 8) {
+            const bool in = block_in && r < valid;
+            ptx::cp_async_4(dst + 4 * (4 * r + j), in ? p.a_scale + static_cast<long long>(row + r) * kb + b0 + j : p.a_scale, in);
+          }
+          const bool in = block_in && 2 * t.nt + r0 < nb;
+          if (r0 < 2) ptx::cp_async_4(dst + 4 * (4 * (128 + r0) + j), in ? sb + static_cast<long long>(r0) * kb + b0 + j : p.b_scale, in);
         }
-        ptx::cp_async_mbar_arrive(sc_full_u32 + 8 * slot);
-        if (++slot == kFp8ScaleSlots) { slot = 0; phase ^= 1; }
+        ptx::cp_async_mbar_arrive(sc_full_u32 + 8 * panel);
+        if (++panel == Cfg::kPanels) { panel = 0; phase ^= 1; }
       }
     }
     ptx::cp_async_wait_all();
@@ -572,7 +605,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     __syncwarp();
   }
   } else {
-    ptx::setmaxnreg_inc<224>();
+    ptx::setmaxnreg_inc<216>();
     // ------------------ promotion: lane = row of the tile, registers = 128 columns (one scale tile of B)
     const int q = warp & 3;
     const int half = (warp - kFirstPromoter) >> 2;
@@ -580,41 +613,49 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t stg = ptx::smem_u32(staging) + (warp - kFirstPromoter) * 4096;
     const uint32_t stg_row = stg + lane * 128;
     const uint32_t sum_empty_target = ptx::map_to_cta(sum_empty_u32, 0);
-    int buf = 0, slot = 0;
-    uint32_t buf_phase = 0, slot_phase = 0;
+    int buf = 0, panel = 0;
+    uint32_t buf_phase = 0, panel_phase = 0;
     bool ok = true;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
       const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
-      float2 acc[64];
+      uint64_t acc[64];                      // column pairs, as the packed FMA takes them
 #pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.0f, 0.0f);
+      for (int c = 0; c < 64; ++c) acc[c] = 0;
+      float4 s4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int b = 0; b < kb; ++b) {
-        if (!ptx::mbar_wait(sc_full_u32 + 8 * slot, slot_phase, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
-        const float* sc = slots + slot * Cfg::kSlotFloats;
-        const float s = sc[q * 32 + lane] * sc[128 + half];
+        if ((b & (Cfg::kPanel - 1)) == 0) {
+          if (!ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
+          const float4* sc = reinterpret_cast<const float4*>(slots + panel * Cfg::kPanelFloats);
+          const float4 sa = sc[q * 32 + lane], sb = sc[128 + half];
+          s4 = make_float4(sa.x * sb.x, sa.y * sb.y, sa.z * sb.z, sa.w * sb.w);
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(sc_empty_u32 + 8 * panel);
+          if (++panel == Cfg::kPanels) { panel = 0; panel_phase ^= 1; }
+        }
+        const uint64_t s = ptx::pack_f32x2(__float_as_uint(s4.x), __float_as_uint(s4.x));
+        s4 = make_float4(s4.y, s4.z, s4.w, s4.x);
         if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
         ptx::tc_fence_after_sync();
+        const uint32_t from = addr + buf * 256;
 #pragma unroll
-        for (int c0 = 0; c0 < 4; ++c0) {
-          uint32_t v[32];
-          ptx::tmem_ld_cols<32>(addr + buf * 256 + c0 * 32, v);
-          ptx::tmem_ld_wait_regs<32>(v);
-          if (c0 == 3) {                       // everything has left tensor memory
+        for (int c0 = 0; c0 < 8; ++c0) {       // 16 columns at a time
+          uint32_t v[16];
+          ptx::tmem_ld_cols<16>(from + c0 * 16, v);
+          ptx::tmem_ld_wait_regs<16>(v);
+          if (c0 == 7) {                       // everything has left tensor memory
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
               if (leader) ptx::mbar_arrive(sum_empty_u32 + 8 * buf);
               else ptx::mbar_arrive_cluster(sum_empty_target + 8 * buf);
-              ptx::mbar_arrive(sc_empty_u32 + 8 * slot);
             }
           }
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
-            acc[c0 * 16 + c] = ptx::fma2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]), s, acc[c0 * 16 + c]);
+          for (int c = 0; c < 8; ++c) ptx::fma_f32x2(acc[c0 * 8 + c], ptx::pack_f32x2(v[2 * c], v[2 * c + 1]), s);
         }
         if (++buf == Cfg::kBuffers) { buf = 0; buf_phase ^= 1; }
-        if (++slot == kFp8ScaleSlots) { slot = 0; slot_phase ^= 1; }
       }
+      auto value = [&](int c) { return __uint_as_float(static_cast<uint32_t>(c & 1 ? acc[c >> 1] >> 32 : acc[c >> 1])); };
       if (!ok) break;
       // ---- output: a slab of 32 valid rows leaves through the staging buffer and the store engine,
       // a ragged one by predicated stores
@@ -624,54 +665,53 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const int col0 = t.nt * 256 + half * 128;
       if (rows_left <= 0 || col0 >= p.n) continue;
       const int elem = p.out_type == kOutF32 ? 4 : 2;
-      const int box = 128 / elem;                        // columns per staged box
       if (p.tma_store && rows_left >= 32) {
 #pragma unroll
         for (int c0 = 0; c0 < 4; ++c0) {                 // 32 columns at a time
           const int col = col0 + c0 * 32;
-          if (col >= p.n) break;
           if (elem == 4 || (c0 & 1) == 0) {
             if (lane == 0) ptx::bulk_wait_group_read<0>();
             __syncwarp();
           }
           if (elem == 4) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              const float2 x = acc[c0 * 16 + 2 * u], y = acc[c0 * 16 + 2 * u + 1];
-              ptx::st_shared_v4(stg_row + (static_cast<uint32_t>(u ^ (lane & 7)) << 4), __float_as_uint(x.x),
-                                __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
-            }
+            for (int u = 0; u < 8; ++u)
+              ptx::st_shared_v4(stg_row + (static_cast<uint32_t>(u ^ (lane & 7)) << 4), __float_as_uint(value(c0 * 32 + 4 * u)),
+                                __float_as_uint(value(c0 * 32 + 4 * u + 1)), __float_as_uint(value(c0 * 32 + 4 * u + 2)),
+                                __float_as_uint(value(c0 * 32 + 4 * u + 3)));
           } else {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               uint32_t w[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = fp8_pack2(p.out_type, acc[c0 * 16 + 4 * u + i].x, acc[c0 * 16 + 4 * u + i].y);
+              for (int i = 0; i < 4; ++i) w[i] = fp8_pack2(p.out_type, value(c0 * 32 + 8 * u + 2 * i), value(c0 * 32 + 8 * u + 2 * i + 1));
               ptx::st_shared_v4(stg_row + (static_cast<uint32_t>(((c0 & 1) * 4 + u) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
           }
-          if (elem == 4 || (c0 & 1) == 1 || col + 32 >= p.n) {
+          if (elem == 4 || (c0 & 1) == 1) {
             ptx::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) {
-              ptx::tma_store_2d(&tmap_out, stg, col0 + (c0 * 32 / box) * box, map_row);
+            const int box_col = elem == 4 ? col : col - 32;
+            if (lane == 0 && box_col < p.n) {
+              ptx::tma_store_2d(&tmap_out, stg, box_col, map_row);
               ptx::bulk_commit_group();
             }
           }
         }
       } else if (lane < rows_left) {
-        const long long at = static_cast<long long>(map_row + lane) * p.n + col0;
+        const long long at = static_cast<long long>(map_row + lane) * p.n;
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {                // 8 columns: n is a multiple of 8
-          if (col0 + 2 * c < p.n) {
+        for (int c = 0; c < 128; c += 8) {               // n is a multiple of 8
+          const int col = col0 + c;
+          if (col < p.n) {
             if (elem == 4) {
-              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + 2 * c);
-              dst[0] = make_float4(acc[c].x, acc[c].y, acc[c + 1].x, acc[c + 1].y);
-              dst[1] = make_float4(acc[c + 2].x, acc[c + 2].y, acc[c + 3].x, acc[c + 3].y);
+              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + col);
+              dst[0] = make_float4(value(c), value(c + 1), value(c + 2), value(c + 3));
+              dst[1] = make_float4(value(c + 4), value(c + 5), value(c + 6), value(c + 7));
             } else {
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + 2 * c) =
-                  make_uint4(fp8_pack2(p.out_type, acc[c].x, acc[c].y), fp8_pack2(p.out_type, acc[c + 1].x, acc[c + 1].y),
-                             fp8_pack2(p.out_type, acc[c + 2].x, acc[c + 2].y), fp8_pack2(p.out_type, acc[c + 3].x, acc[c + 3].y));
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + col) =
+                  make_uint4(fp8_pack2(p.out_type, value(c), value(c + 1)), fp8_pack2(p.out_type, value(c + 2), value(c + 3)),
+                             fp8_pack2(p.out_type, value(c + 4), value(c + 5)), fp8_pack2(p.out_type, value(c + 6), value(c + 7)));
             }
           }
         }

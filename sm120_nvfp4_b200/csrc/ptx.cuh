@@ -409,18 +409,14 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-// acc + {x, y} * {s, s}: two FP32 fused multiply-adds in one instruction.
-__device__ __forceinline__ float2 fma2(float x, float y, float s, float2 acc) {
-  float2 r;
-  asm("{\n\t.reg .b64 a, b, c;\n\t"
-      "mov.b64 a, {%2, %3};\n\t"
-      "mov.b64 b, {%4, %4};\n\t"
-      "mov.b64 c, {%5, %6};\n\t"
-      "fma.rn.f32x2 c, a, b, c;\n\t"
-      "mov.b64 {%0, %1}, c;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(x), "f"(y), "f"(s), "f"(acc.x), "f"(acc.y));
+// acc += a * b on two FP32 lanes packed into 64 bits: two fused multiply-adds in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
   return r;
+}
+__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 
 // Register shares of the warpgroups of a block: all four warps of a warpgroup execute it, and the
@@ -440,6 +436,12 @@ __device__ __forceinline__ void setmaxnreg_inc() {
 __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const float* src, bool read) {
   const uint32_t bytes = read ? 4u : 0u;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// 16 bytes, both addresses 16-byte aligned.
+__device__ __forceinline__ void cp_async_16(uint32_t smem_dst, const float* src, bool read) {
+  const uint32_t bytes = read ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // This thread's arrival on `bar` once all its earlier copies have landed.
