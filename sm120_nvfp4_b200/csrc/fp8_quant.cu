@@ -17,10 +17,10 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 
 #include "host_common.hpp"
 #include "internal.hpp"
-#include "nvfp4_math.cuh"
 
 namespace b200 {
 namespace {
@@ -67,22 +67,47 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   return lo | (hi << 16);
 }
 
+// v[j] / s for a divisor whose correctly rounded reciprocal is y: Markstein's sequence (see above). The
+// signs are chosen so that a quotient of -0 stays -0.
+__device__ __forceinline__ float quotient(float v, float s, float y) {
+  const float q0 = __fmul_rn(v, y);
+  return __fmaf_rn(-__fmaf_rn(q0, s, -v), y, q0);
+}
+
+// silu(g) * u = g / (1 + e^-g) * u in IEEE FP32 steps. Inside |g| <= 87 the divisor lies in [1, 2^126], so
+// the quotient needs no special cases; outside (or infinite) the eight values take the plain division.
+__device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+  if (top <= 87.0f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = __fadd_rn(1.0f, expf(-v[j]));
+      v[j] = __fmul_rn(quotient(v[j], d, __frcp_rn(d)), u[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))), u[j]);
+  }
+}
+
+// `step_rows`, `step_cols`: 16 / kb and 16 % kb, the way from one of a thread's blocks to its next.
 template <typename T, bool kSwiglu, int kUnroll>
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T* __restrict__ x, int k, uint32_t kb,
-                    uint32_t blocks) {
+                    uint32_t blocks, uint32_t step_rows, uint32_t step_cols) {
   const int lane = threadIdx.x & 15;
   const uint32_t first = blockIdx.x * (16u * kUnroll) + (threadIdx.x >> 4);
   float v[kUnroll][8];
   [[maybe_unused]] float u[kUnroll][8];
   long long at[kUnroll];
   bool in[kUnroll];
+  uint32_t row = first / kb, col_block = first - row * kb;
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
-    const uint32_t block = first + 16u * i;
-    const uint32_t row = block / kb;
-    const int col = static_cast<int>(block - row * kb) * 128 + lane * 8;
-    in[i] = block < blocks && col < k;
+    const int col = static_cast<int>(col_block) * 128 + lane * 8;
+    in[i] = first + 16u * i < blocks && col < k;
     at[i] = static_cast<long long>(row) * k + col;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
@@ -95,16 +120,14 @@ fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T*
         load8(x + at[i], v[i]);
       }
     }
+    row += step_rows;
+    col_block += step_cols;
+    if (col_block >= kb) { col_block -= kb; ++row; }
   }
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
     if constexpr (kSwiglu) {
-      if (in[i]) {
-        float g[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = v[i][j];
-        silu_mul_block(g, u[i], v[i]);
-      }
+      if (in[i]) silu_mul8(v[i], u[i]);
     }
     float amax = kAmaxFloor;
 #pragma unroll
@@ -112,35 +135,37 @@ fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T*
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     const float s = __fdiv_rn(amax, kE4m3Max);
-    float r[8];
     if (s < __int_as_float(0x7f800000)) {
       const float y = __frcp_rn(s);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q0 = __fmul_rn(v[i][j], y);
-        const float e = __fmaf_rn(__fmaf_rn(-q0, s, v[i][j]), y, q0);
-        r[j] = copysignf(e, v[i][j]);     // a zero remainder would turn -0 into +0
-      }
+      for (int j = 0; j < 8; ++j) v[i][j] = quotient(v[i][j], s, y);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = __fdiv_rn(v[i][j], s);
+      for (int j = 0; j < 8; ++j) v[i][j] = __fdiv_rn(v[i][j], s);
     }
     if (in[i]) {
-      *reinterpret_cast<uint2*>(q + at[i]) = make_uint2(pack4(r[0], r[1], r[2], r[3]), pack4(r[4], r[5], r[6], r[7]));
+      *reinterpret_cast<uint2*>(q + at[i]) =
+          make_uint2(pack4(v[i][0], v[i][1], v[i][2], v[i][3]), pack4(v[i][4], v[i][5], v[i][6], v[i][7]));
       if (lane == 0) scale[first + 16u * i] = s;
     }
   }
 }
 
+template <typename T, bool kSwiglu, int kUnroll>
+void launch_blocks(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, cudaStream_t stream) {
+  constexpr uint32_t kPerBlock = 16u * kUnroll;
+  fp8_quantize_kernel<T, kSwiglu, kUnroll><<<(blocks + kPerBlock - 1) / kPerBlock, 256, 0, stream>>>(
+      static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks, 16u / kb, 16u % kb);
+}
+
 template <typename T, bool kSwiglu>
 void launch_quantize(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, int sms, cudaStream_t stream) {
-  // four blocks of 128 per sixteen lanes once that still leaves every SM two thread blocks, else one
-  if (blocks >= static_cast<uint32_t>(sms) * 2u * 64u)
-    fp8_quantize_kernel<T, kSwiglu, 4><<<(blocks + 63u) / 64u, 256, 0, stream>>>(
-        static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks);
+  // several blocks of 128 per sixteen lanes once that still leaves every SM two thread blocks, else one
+  constexpr int kUnroll = kSwiglu ? 1 : 2;
+  if (blocks >= static_cast<uint32_t>(sms) * 2u * 16u * kUnroll)
+    launch_blocks<T, kSwiglu, kUnroll>(q, scale, x, k, kb, blocks, stream);
   else
-    fp8_quantize_kernel<T, kSwiglu, 1><<<(blocks + 15u) / 16u, 256, 0, stream>>>(
-        static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks);
+    launch_blocks<T, kSwiglu, 1>(q, scale, x, k, kb, blocks, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
