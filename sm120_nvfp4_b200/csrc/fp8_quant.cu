@@ -3,9 +3,9 @@
 //   amax_b = max(|x|) over the 128 values of a block, at least 2^-60
 //   s_b = RN(amax_b / 448),  q = E4M3(RN(x / s_b))
 //
-// HBM-bound: 2 bytes read (4 with SiLU) and 1.03 written per value of a 16-bit input. Sixteen lanes
-// share a block, eight values each: one 16-byte load (two for FP32), an amax by four shuffles and one
-// 8-byte store, all coalesced; a thread works on several blocks so that their loads overlap.
+// HBM-bound: 2 bytes read (4 with SiLU) and 1.03 written per value of a 16-bit input; with SiLU the
+// arithmetic - an exponential and a division per value - comes close. Eight (or sixteen) lanes share a
+// block: 16-byte loads, an amax by three (four) exchanges, one 16-byte (8-byte) store.
 //
 // The division: every quotient of a block has the same divisor s, so one correctly rounded reciprocal
 // r = RN(1 / s) serves them all by Markstein's sequence (IBM J. Res. Dev. 34(1), 1990): q0 = RN(x r),
@@ -34,31 +34,43 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+// N consecutive values (a multiple of 8 for 16-bit types, of 4 for FP32) in 16-byte loads.
+template <int N>
+__device__ __forceinline__ void load(const __half* p, float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+  for (int c = 0; c < N / 8; ++c) {
+    const uint4 w = reinterpret_cast<const uint4*>(p)[c];
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+      v[8 * c + 2 * i] = f.x;
+      v[8 * c + 2 * i + 1] = f.y;
+    }
   }
 }
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+template <int N>
+__device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(a[i] << 16);
-    v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+  for (int c = 0; c < N / 8; ++c) {
+    const uint4 w = reinterpret_cast<const uint4*>(p)[c];
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[8 * c + 2 * i] = __uint_as_float(a[i] << 16);
+      v[8 * c + 2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+    }
   }
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+template <int N>
+__device__ __forceinline__ void load(const float* p, float (&v)[N]) {
+#pragma unroll
+  for (int c = 0; c < N / 4; ++c) {
+    const float4 a = reinterpret_cast<const float4*>(p)[c];
+    v[4 * c] = a.x; v[4 * c + 1] = a.y; v[4 * c + 2] = a.z; v[4 * c + 3] = a.w;
+  }
 }
 
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
@@ -67,57 +79,74 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   return lo | (hi << 16);
 }
 
-// v[j] / s for a divisor whose correctly rounded reciprocal is y: Markstein's sequence (see above). The
-// signs are chosen so that a quotient of -0 stays -0.
-__device__ __forceinline__ float quotient(float v, float s, float y) {
-  const float q0 = __fmul_rn(v, y);
-  return __fmaf_rn(-__fmaf_rn(q0, s, -v), y, q0);
+// Two FP32 operations in one instruction (each lane rounds as the scalar one would).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
-// silu(g) * u = g / (1 + e^-g) * u in IEEE FP32 steps. Inside |g| <= 87 the divisor lies in [1, 2^126], so
-// the quotient needs no special cases; outside (or infinite) the eight values take the plain division.
-__device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
-  float top = 0.0f;
+// v -> -(v / s) for N values whose divisor has the correctly rounded reciprocal y: Markstein's sequence (see
+// above). Computed with its sign turned round because then a quotient of -0 stays a zero of the right
+// sign; the caller turns the codes' signs back.
+template <int N>
+__device__ __forceinline__ void minus_quotients(float (&v)[N], float s, float y) {
+  const uint64_t s2 = pack2(s, s), y2 = pack2(-y, -y);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
-  if (top <= 87.0f) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = __fadd_rn(1.0f, expf(-v[j]));
-      v[j] = __fmul_rn(quotient(v[j], d, __frcp_rn(d)), u[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))), u[j]);
+  for (int j = 0; j < N; j += 2) {
+    const uint64_t x = pack2(v[j], v[j + 1]);
+    const uint64_t q0 = mul2(x, y2);
+    unpack2(fma2(fma2(q0, s2, x), y2, q0), v[j], v[j + 1]);
   }
 }
 
-// `step_rows`, `step_cols`: 16 / kb and 16 % kb, the way from one of a thread's blocks to its next.
-template <typename T, bool kSwiglu, int kUnroll>
+// silu(g) * u = g / (1 + e^-g) * u in IEEE FP32 steps.
+template <int N>
+__device__ __forceinline__ void silu_mul(float (&v)[N], const float (&u)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = __fmul_rn(__fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))), u[j]);
+}
+
+// kPer values per thread: 128 / kPer lanes share a block of 128. `step_rows`, `step_cols`: how far the next of a
+// thread's kUnroll blocks is, in rows and blocks (the blocks a thread block handles at a time / kb, % kb).
+template <typename T, bool kSwiglu, int kPer, int kUnroll>
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T* __restrict__ x, int k, uint32_t kb,
                     uint32_t blocks, uint32_t step_rows, uint32_t step_cols) {
-  const int lane = threadIdx.x & 15;
-  const uint32_t first = blockIdx.x * (16u * kUnroll) + (threadIdx.x >> 4);
-  float v[kUnroll][8];
-  [[maybe_unused]] float u[kUnroll][8];
+  constexpr int kLanes = 128 / kPer;
+  constexpr uint32_t kAtOnce = 256 / kLanes;
+  const int lane = threadIdx.x & (kLanes - 1);
+  const uint32_t first = blockIdx.x * (kAtOnce * kUnroll) + threadIdx.x / kLanes;
+  float v[kUnroll][kPer];
+  [[maybe_unused]] float u[kSwiglu ? kUnroll : 1][kPer];
   long long at[kUnroll];
   bool in[kUnroll];
   uint32_t row = first / kb, col_block = first - row * kb;
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
-    const int col = static_cast<int>(col_block) * 128 + lane * 8;
-    in[i] = first + 16u * i < blocks && col < k;
+    const int col = static_cast<int>(col_block) * 128 + lane * kPer;
+    in[i] = first + kAtOnce * i < blocks && col < k;
     at[i] = static_cast<long long>(row) * k + col;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    for (int j = 0; j < kPer; ++j) v[i][j] = 0.0f;
     if (in[i]) {
       if constexpr (kSwiglu) {
         const T* src = x + at[i] + static_cast<long long>(row) * k;     // rows of 2 k: gate, then up
-        load8(src, v[i]);
-        load8(src + k, u[i]);
+        load(src, v[i]);
+        load(src + k, u[i]);
       } else {
-        load8(x + at[i], v[i]);
+        load(x + at[i], v[i]);
       }
     }
     row += step_rows;
@@ -127,45 +156,52 @@ fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T*
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
     if constexpr (kSwiglu) {
-      if (in[i]) silu_mul8(v[i], u[i]);
+      if (in[i]) silu_mul(v[i], u[i]);
     }
     float amax = kAmaxFloor;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i][j]));
+    for (int j = 0; j < kPer; ++j) amax = max_nan(amax, fabsf(v[i][j]));
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    for (int d = kLanes / 2; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     const float s = __fdiv_rn(amax, kE4m3Max);
     if (s < __int_as_float(0x7f800000)) {
       const float y = __frcp_rn(s);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = quotient(v[i][j], s, y);
+      minus_quotients(v[i], s, y);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = __fdiv_rn(v[i][j], s);
+      for (int j = 0; j < kPer; ++j) v[i][j] = -__fdiv_rn(v[i][j], s);
     }
     if (in[i]) {
-      *reinterpret_cast<uint2*>(q + at[i]) =
-          make_uint2(pack4(v[i][0], v[i][1], v[i][2], v[i][3]), pack4(v[i][4], v[i][5], v[i][6], v[i][7]));
-      if (lane == 0) scale[first + 16u * i] = s;
+      uint32_t w[kPer / 4];
+#pragma unroll
+      for (int j = 0; j < kPer / 4; ++j) w[j] = pack4(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]) ^ 0x80808080u;
+      if constexpr (kPer == 16) *reinterpret_cast<uint4*>(q + at[i]) = make_uint4(w[0], w[1], w[2], w[3]);
+      else *reinterpret_cast<uint2*>(q + at[i]) = make_uint2(w[0], w[1]);
+      if (lane == 0) scale[first + kAtOnce * i] = s;
     }
   }
 }
 
-template <typename T, bool kSwiglu, int kUnroll>
+template <typename T, bool kSwiglu, int kPer, int kUnroll>
 void launch_blocks(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, cudaStream_t stream) {
-  constexpr uint32_t kPerBlock = 16u * kUnroll;
-  fp8_quantize_kernel<T, kSwiglu, kUnroll><<<(blocks + kPerBlock - 1) / kPerBlock, 256, 0, stream>>>(
-      static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks, 16u / kb, 16u % kb);
+  constexpr uint32_t kAtOnce = 256u * kPer / 128u, kPerBlock = kAtOnce * kUnroll;
+  fp8_quantize_kernel<T, kSwiglu, kPer, kUnroll><<<(blocks + kPerBlock - 1) / kPerBlock, 256, 0, stream>>>(
+      static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks, kAtOnce / kb, kAtOnce % kb);
 }
 
 template <typename T, bool kSwiglu>
 void launch_quantize(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, int sms, cudaStream_t stream) {
-  // several blocks of 128 per sixteen lanes once that still leaves every SM two thread blocks, else one
-  constexpr int kUnroll = kSwiglu ? 1 : 2;
-  if (blocks >= static_cast<uint32_t>(sms) * 2u * 16u * kUnroll)
-    launch_blocks<T, kSwiglu, kUnroll>(q, scale, x, k, kb, blocks, stream);
+  // Sixteen values per thread halve what a block costs beside its values (index, exchanges, scale); eight
+  // where that leaves SMs idle, and for FP32, whose loads would be strided further apart (16384 x 4096: 53.4
+  // us with sixteen and one block, 51.3 with eight and two). More blocks per thread cost more
+  // occupancy than their overlapped loads bring: 32768 x 4096 BF16 74 us with one, 86 with two; with SiLU
+  // 32768 x 2048 88 and 109.
+  constexpr int kPer = sizeof(T) == 2 ? 16 : 8;
+  constexpr int kUnroll = sizeof(T) == 4 && !kSwiglu ? 2 : 1;
+  if (blocks >= static_cast<uint32_t>(sms) * 2u * 2u * kPer * kUnroll)
+    launch_blocks<T, kSwiglu, kPer, kUnroll>(q, scale, x, k, kb, blocks, stream);
   else
-    launch_blocks<T, kSwiglu, 1>(q, scale, x, k, kb, blocks, stream);
+    launch_blocks<T, kSwiglu, 8, 1>(q, scale, x, k, kb, blocks, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
