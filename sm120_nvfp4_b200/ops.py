@@ -620,21 +620,33 @@ _FP8_OUT = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 _INPUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _launch(device: torch.device, function: str, *args) -> None:
-    """Calls a C-ABI function with torch's current stream of `device` as its last argument; the device is
-    switched only where it is not the current one."""
+# The checks below run on every call, and a small call is all checks and launch: they read integers, build no
+# messages unless one is needed, and take the stream and device by their raw numbers.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _launch(index: int, function: str, *args) -> None:
+    """Calls a C-ABI function with torch's current stream of device `index` as its last argument; the device
+    is switched only where it is not the current one."""
     call = getattr(_lib.lib(), function)
-    if torch.cuda.current_device() == device.index:
-        status = call(*args, _stream(device))
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
+        status = call(*args, stream)
     else:
-        with torch.cuda.device(device):
-            status = call(*args, _stream(device))
+        with torch.cuda.device(index):
+            status = call(*args, stream)
     if status:
         raise RuntimeError(f"{function} failed: {_lib.status_string(status)}")
 
 
-def _is_fp8(t: torch.Tensor) -> bool:
-    return t.dtype == _FP8 or t.dtype == torch.uint8
+def _on_device(index: int, tensors, names) -> None:
+    """Every tensor is a contiguous CUDA tensor on device `index`."""
+    for t, name in zip(tensors, names):
+        if not (t.is_cuda and t.get_device() == index and t.is_contiguous()):
+            _check_cuda_contig(t, torch.device("cuda", index), name)
+
+
+_FP8_STORAGE = (_FP8, torch.uint8)
 
 
 def _blocks_128(n: int) -> int:
@@ -651,58 +663,64 @@ def quantize_fp8(x: torch.Tensor, *, swiglu: bool = False, output: Optional[torc
     step between the two products of an expert. A block with a NaN or an infinity gets a NaN or
     infinite scale. Not differentiable.
     """
-    _check(x.is_cuda and x.dim() == 2 and x.is_contiguous() and x.dtype in _INPUT,
-           "x must be a contiguous FP16, BF16 or FP32 CUDA matrix")
+    kind = _INPUT.get(x.dtype)
+    if not (kind is not None and x.is_cuda and x.dim() == 2 and x.is_contiguous()):
+        _check(False, "x must be a contiguous FP16, BF16 or FP32 CUDA matrix")
     rows, k = x.shape
     if swiglu:
         _check(k % 2 == 0, "x must hold gate and up columns")
         k //= 2
     _check(k > 0 and k % 16 == 0, "K must be a positive multiple of 16")
-    _check(x.data_ptr() % 16 == 0, "x must be 16-byte aligned")
-    device = x.device
+    source = x.data_ptr()
+    _check(source % 16 == 0, "x must be 16-byte aligned")
+    index = x.get_device()
     if output is None:
-        output = torch.empty((rows, k), dtype=_FP8, device=device)
+        output = x.new_empty((rows, k), dtype=_FP8)
     else:
-        _check_cuda_contig(output, device, "output")
-        _check(_is_fp8(output) and tuple(output.shape) == (rows, k) and output.data_ptr() % 16 == 0,
+        _on_device(index, (output,), ("output",))
+        _check(output.dtype in _FP8_STORAGE and output.shape == (rows, k) and output.data_ptr() % 16 == 0,
                "output must be 16-byte aligned float8_e4m3fn (or uint8) [rows, K]")
     if output_scale is None:
-        output_scale = torch.empty((rows, _blocks_128(k)), dtype=torch.float32, device=device)
+        output_scale = x.new_empty((rows, _blocks_128(k)), dtype=torch.float32)
     else:
-        _check_cuda_contig(output_scale, device, "output_scale")
-        _check(output_scale.dtype == torch.float32 and tuple(output_scale.shape) == (rows, _blocks_128(k)),
+        _on_device(index, (output_scale,), ("output_scale",))
+        _check(output_scale.dtype == torch.float32 and output_scale.shape == (rows, _blocks_128(k)),
                "output_scale must be float32 [rows, ceil(K/128)]")
     if rows:
-        _launch(device, "b200_nvfp4_fp8_quantize_rows", output.data_ptr(), output_scale.data_ptr(), x.data_ptr(), rows, k,
-                _INPUT[x.dtype], int(swiglu))
+        _launch(index, "b200_nvfp4_fp8_quantize_rows", output.data_ptr(), output_scale.data_ptr(), source, rows, k, kind,
+                int(swiglu))
     return output, output_scale
 
 
 def _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output, names):
-    device = x.device
-    for t, name in zip((x, weight, x_scale, weight_scale), names):
-        _check_cuda_contig(t, device, name)
-    _check(_is_fp8(x) and _is_fp8(weight), f"{names[0]} and {names[1]} must be float8_e4m3fn (or raw uint8 codes)")
+    index = x.get_device()
+    _on_device(index, (x, weight, x_scale, weight_scale), names)
+    if x.dtype not in _FP8_STORAGE or weight.dtype not in _FP8_STORAGE:
+        _check(False, f"{names[0]} and {names[1]} must be float8_e4m3fn (or raw uint8 codes)")
     _check(x_scale.dtype == torch.float32 and weight_scale.dtype == torch.float32, "scales must be float32")
-    _check(x.dim() == 2 and x.size(1) == weight.size(-1), f"{names[0]} and {names[1]} must share K")
-    rows, k = x.shape
-    n = weight.size(-2)
+    shape = weight.shape
+    n, k = shape[-2], shape[-1]
+    if x.dim() != 2 or x.shape[1] != k:
+        _check(False, f"{names[0]} and {names[1]} must share K")
+    rows = x.shape[0]
     _check(k > 0 and k % 16 == 0, "K must be a positive multiple of 16")
     _check(n > 0 and n % 8 == 0, "N must be a positive multiple of 8")
     kb = _blocks_128(k)
-    _check(tuple(x_scale.shape) == (rows, kb), f"{names[2]} must be [rows, ceil(K/128)]")
-    _check(tuple(weight_scale.shape) == (*weight.shape[:-2], _blocks_128(n), kb),
-           f"{names[3]} must hold one scale per 128 x 128 block of {names[1]}")
-    _check(x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0, f"{names[0]} and {names[1]} must be 16-byte aligned")
+    if x_scale.shape != (rows, kb):
+        _check(False, f"{names[2]} must be [rows, ceil(K/128)]")
+    if weight_scale.shape != (*shape[:-2], _blocks_128(n), kb):
+        _check(False, f"{names[3]} must hold one scale per 128 x 128 block of {names[1]}")
+    if x.data_ptr() % 16 or weight.data_ptr() % 16:
+        _check(False, f"{names[0]} and {names[1]} must be 16-byte aligned")
     if output is None:
         _check(out_dtype in _FP8_OUT, "out_dtype must be float16, bfloat16 or float32")
-        output = torch.empty((rows, n), dtype=out_dtype, device=device)
+        output = x.new_empty((rows, n), dtype=out_dtype)
     else:
-        _check_cuda_contig(output, device, "output")
-        _check(output.dtype in _FP8_OUT and tuple(output.shape) == (rows, n) and output.data_ptr() % 16 == 0,
+        _on_device(index, (output,), ("output",))
+        _check(output.dtype in _FP8_OUT and output.shape == (rows, n) and output.data_ptr() % 16 == 0,
                "output must be a 16-byte aligned FP16, BF16 or FP32 matrix [rows, N]")
         _check(out_dtype is None or out_dtype == output.dtype, "out_dtype does not match output")
-    return rows, n, k, output
+    return index, rows, n, k, output
 
 
 def fp8_gemm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, *,
@@ -720,9 +738,9 @@ def fp8_gemm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: t
     _check(b.dim() == 2, "b must be [N, K]")
     if out_dtype is None and output is None:
         out_dtype = torch.float16
-    m, n, k, out = _fp8_operands(a, b, a_scale, b_scale, out_dtype, output, ("a", "b", "a_scale", "b_scale"))
+    index, m, n, k, out = _fp8_operands(a, b, a_scale, b_scale, out_dtype, output, ("a", "b", "a_scale", "b_scale"))
     if m:
-        _launch(a.device, "b200_nvfp4_fp8_gemm", m, n, k, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
+        _launch(index, "b200_nvfp4_fp8_gemm", m, n, k, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
                 out.data_ptr(), _FP8_OUT[out.dtype])
     return out
 
@@ -740,17 +758,16 @@ def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tenso
     _check(weight.dim() == 3, "weight must be [groups, N, K]")
     if out_dtype is None and output is None:
         out_dtype = torch.float16
-    rows, n, k, out = _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output,
-                                    ("x", "weight", "x_scale", "weight_scale"))
-    groups = weight.size(0)
+    index, rows, n, k, out = _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output,
+                                           ("x", "weight", "x_scale", "weight_scale"))
+    groups = weight.shape[0]
     _check(0 < groups <= 256, "number of groups must be in [1, 256]")
-    for t, name in ((seqlens, "seqlens"), (cu_seqlens, "cu_seqlens")):
-        _check_cuda_contig(t, x.device, name)
-        _check(t.dtype == torch.int32, "seqlens and cu_seqlens must be int32")
+    _on_device(index, (seqlens, cu_seqlens), ("seqlens", "cu_seqlens"))
+    _check(seqlens.dtype == torch.int32 and cu_seqlens.dtype == torch.int32, "seqlens and cu_seqlens must be int32")
     _check(seqlens.numel() == groups and cu_seqlens.numel() == groups + 1,
            "seqlens / cu_seqlens lengths are inconsistent with the number of groups")
     if rows:
-        _launch(x.device, "b200_nvfp4_fp8_grouped_gemm", out.data_ptr(), x.data_ptr(), weight.data_ptr(), seqlens.data_ptr(),
+        _launch(index, "b200_nvfp4_fp8_grouped_gemm", out.data_ptr(), x.data_ptr(), weight.data_ptr(), seqlens.data_ptr(),
                 cu_seqlens.data_ptr(), x_scale.data_ptr(), weight_scale.data_ptr(), groups, rows, n, k, 0,
                 _FP8_OUT[out.dtype])
     return out
@@ -763,33 +780,35 @@ _SCORING = {"sigmoid": 0, "softmax": 1}
 
 
 def _check_router(logits, topk_ids, cu_seqlens, scoring):
-    _check(logits.is_cuda and logits.dim() == 2 and logits.is_contiguous() and logits.dtype in _INPUT,
-           "logits must be a contiguous FP32, BF16 or FP16 CUDA tensor [num_tokens, num_experts]")
+    kind = _INPUT.get(logits.dtype)
+    if not (kind is not None and logits.is_cuda and logits.dim() == 2 and logits.is_contiguous()):
+        _check(False, "logits must be a contiguous FP32, BF16 or FP16 CUDA tensor [num_tokens, num_experts]")
     t, e = logits.shape
-    _check_cuda_contig(topk_ids, logits.device, "topk_ids")
-    _check(topk_ids.dtype == torch.int32 and topk_ids.dim() == 2 and topk_ids.size(0) == t,
+    index = logits.get_device()
+    _on_device(index, (topk_ids,), ("topk_ids",))
+    _check(topk_ids.dtype == torch.int32 and topk_ids.dim() == 2 and topk_ids.shape[0] == t,
            "topk_ids must be int32 [num_tokens, num_topk]")
-    _check(0 < topk_ids.size(1) <= e <= 4096, "need 0 < num_topk <= num_experts <= 4096")
+    k = topk_ids.shape[1]
+    _check(0 < k <= e <= 4096, "need 0 < num_topk <= num_experts <= 4096")
     _check(scoring in _SCORING, "scoring must be 'sigmoid' or 'softmax'")
     sequences = 1
     if cu_seqlens is not None:
-        _check_cuda_contig(cu_seqlens, logits.device, "cu_seqlens")
+        _on_device(index, (cu_seqlens,), ("cu_seqlens",))
         _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 2 <= cu_seqlens.numel() <= 65537,
                "cu_seqlens must be int32 [num_sequences + 1] with at most 65536 sequences")
         sequences = cu_seqlens.numel() - 1
-    return t, e, topk_ids.size(1), sequences
+    return index, kind, t, e, k, sequences
 
 
 def _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha):
-    t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
-    device = logits.device
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    counts = torch.empty((sequences, e), dtype=torch.int32, device=device)
-    slope = torch.empty((sequences, e), dtype=torch.float32, device=device)
+    index, kind, t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
+    loss = logits.new_empty((), dtype=torch.float32)
+    counts = topk_ids.new_empty((sequences, e))
+    slope = logits.new_empty((sequences, e), dtype=torch.float32)
     need = _lib.lib().b200_nvfp4_moe_balance_loss_workspace_bytes(t, e, sequences)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _launch(device, "b200_nvfp4_moe_balance_loss", loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), logits.data_ptr(),
-            topk_ids.data_ptr(), _ptr(cu_seqlens), t, e, k, sequences, _INPUT[logits.dtype], _SCORING[scoring], float(alpha),
+    workspace = logits.new_empty(need, dtype=torch.uint8)
+    _launch(index, "b200_nvfp4_moe_balance_loss", loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), logits.data_ptr(),
+            topk_ids.data_ptr(), _ptr(cu_seqlens), t, e, k, sequences, kind, _SCORING[scoring], float(alpha),
             workspace.data_ptr(), need)
     return loss, counts, slope
 
@@ -806,26 +825,26 @@ def router_backward(logits: torch.Tensor, topk_ids: torch.Tensor, *, topk_weight
     `scoring` is that of the loss; the weights are router_topk's (sigmoid). Slots with an id outside
     [0, E) are empty; slots of a token that name the same expert add up.
     """
-    t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
+    index, kind, t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
     _check(grad_weights is not None or slope is not None, "grad_weights or slope must be given")
-    device = logits.device
     if grad_weights is not None:
         _check(topk_weights is not None, "grad_weights needs topk_weights")
-        for x, name in ((topk_weights, "topk_weights"), (grad_weights, "grad_weights")):
-            _check_cuda_contig(x, device, name)
-            _check(x.dtype == torch.float32 and x.shape == topk_ids.shape, "topk_weights and grad_weights must be float32 [T, k]")
+        _on_device(index, (topk_weights, grad_weights), ("topk_weights", "grad_weights"))
+        _check(topk_weights.dtype == torch.float32 and grad_weights.dtype == torch.float32 and
+               topk_weights.shape == topk_ids.shape and grad_weights.shape == topk_ids.shape,
+               "topk_weights and grad_weights must be float32 [T, k]")
     if slope is not None:
         _check(grad_loss is not None, "slope needs grad_loss")
-        _check_cuda_contig(slope, device, "slope")
-        _check(slope.dtype == torch.float32 and tuple(slope.shape) == (sequences, e),
+        _on_device(index, (slope,), ("slope",))
+        _check(slope.dtype == torch.float32 and slope.shape == (sequences, e),
                "slope must be float32 [num_sequences, num_experts]")
-        _check(grad_loss.is_cuda and grad_loss.device == device and grad_loss.dtype == torch.float32 and grad_loss.numel() == 1,
-               "grad_loss must be one float32 on the device of the logits")
+        _check(grad_loss.is_cuda and grad_loss.get_device() == index and grad_loss.dtype == torch.float32 and
+               grad_loss.numel() == 1, "grad_loss must be one float32 on the device of the logits")
     grad = torch.empty_like(logits)
     if t:
-        _launch(device, "b200_nvfp4_moe_router_backward", grad.data_ptr(), logits.data_ptr(), topk_ids.data_ptr(),
+        _launch(index, "b200_nvfp4_moe_router_backward", grad.data_ptr(), logits.data_ptr(), topk_ids.data_ptr(),
                 _ptr(topk_weights), _ptr(grad_weights), _ptr(slope), _ptr(grad_loss) if slope is not None else None,
-                _ptr(cu_seqlens), t, e, k, sequences, _INPUT[logits.dtype], _SCORING[scoring])
+                _ptr(cu_seqlens), t, e, k, sequences, kind, _SCORING[scoring])
     return grad
 
 
