@@ -58,10 +58,10 @@ long long row_tiles(const Fp8Problem& q, int tile_rows) {
   return q.seqlens == nullptr ? exact : static_cast<long long>(q.rows) / tile_rows + (q.rows < q.groups ? q.rows : q.groups);
 }
 
-template <int BN>
+template <int BN, bool kWide>
 int launch_skinny(const Fp8Problem& q, Fp8Params p, int splits, const DeviceInfo& dev, cudaStream_t stream) {
-  using Cfg = Fp8SkinnyCfg<BN>;
-  auto kernel = fp8_skinny_kernel<BN>;
+  using Cfg = Fp8SkinnyCfg<BN, kWide>;
+  auto kernel = fp8_skinny_kernel<BN, kWide>;
   static std::once_flag once[64];
   static cudaError_t attr_status[64];
   std::call_once(once[dev.device], [&] {
@@ -69,15 +69,15 @@ int launch_skinny(const Fp8Problem& q, Fp8Params p, int splits, const DeviceInfo
   });
   if (attr_status[dev.device] != cudaSuccess) return B200_NVFP4_CUDA_ERROR;
   CUtensorMap tmap_x, tmap_w;
-  if (!encode_tmap_2d_u8(&tmap_x, q.a, static_cast<uint64_t>(q.rows), static_cast<uint64_t>(q.k), BN, kFp8BlockK,
+  if (!encode_tmap_2d_u8(&tmap_x, q.a, static_cast<uint64_t>(q.rows), static_cast<uint64_t>(q.k), Cfg::kTileM, kFp8BlockK,
                          CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !encode_tmap_2d_u8(&tmap_w, q.b, static_cast<uint64_t>(q.groups) * q.n, static_cast<uint64_t>(q.k), 128, kFp8BlockK,
+      !encode_tmap_2d_u8(&tmap_w, q.b, static_cast<uint64_t>(q.groups) * q.n, static_cast<uint64_t>(q.k), Cfg::kTileN, kFp8BlockK,
                          CU_TENSOR_MAP_SWIZZLE_128B))
     return B200_NVFP4_CUDA_ERROR;
   p.splits = splits;
   p.num_stages = Cfg::stages_for(q.groups, splits);
   p.raster_m = 16;
-  const long long tasks = row_tiles(q, BN) * ((q.n + 127) / 128);
+  const long long tasks = row_tiles(q, Cfg::kTileM) * ((q.n + Cfg::kTileN - 1) / Cfg::kTileN);
   const long long blocks = splits > 1 ? tasks * splits : (tasks < dev.sm_count ? tasks : dev.sm_count);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks));
@@ -107,7 +107,7 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
     cudaFuncAttributes attr;
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, fp8_pair_kernel);
     // the kernel moves registers between its warpgroups: it must have been launched with all of them
-    if (e == cudaSuccess && attr.numRegs * Cfg::kThreads < 72 * 128 + 216 * 256) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess && attr.numRegs * Cfg::kThreads < 104 * 128 + 200 * 256) e = cudaErrorInvalidConfiguration;
     attr_status[dev.device] = e;
     max_pairs[dev.device] = e == cudaSuccess ? resident_clusters(fp8_pair_kernel, dev, 2, Cfg::kThreads, kSmemBudget) : 0;
   });
@@ -180,10 +180,10 @@ int fp8_product(const Fp8Problem& q, const void* a_scale, const void* b_scale, v
   int splits = g_fp8_splits.load(std::memory_order_relaxed);
   if (splits == 0) splits = pick_fp8_splits(q, dev, tile);
   switch (tile) {
-    case 16: return launch_skinny<16>(q, p, splits, dev, stream);
-    case 32: return launch_skinny<32>(q, p, splits, dev, stream);
-    case 64: return launch_skinny<64>(q, p, splits, dev, stream);
-    default: return launch_skinny<128>(q, p, splits, dev, stream);
+    case 16: return launch_skinny<16, false>(q, p, splits, dev, stream);
+    case 32: return launch_skinny<32, false>(q, p, splits, dev, stream);
+    case 64: return launch_skinny<64, false>(q, p, splits, dev, stream);
+    default: return launch_skinny<128, true>(q, p, splits, dev, stream);
   }
 }
 

@@ -14,14 +14,19 @@
 // of these block sums, so the promotion of one block runs under the MMAs of the next.
 //
 // Two kernels:
-//   fp8_skinny_kernel<BN>  few rows. The weights take the 128-row side of the MMA and BN = 16 .. 128
+//   fp8_skinny_kernel<BN, kWide>  few rows; K can be split over a cluster whose CTAs add their partial
+//                          tiles through distributed shared memory, in split order.
+//                          kWide = false: the weights take the 128-row side of the MMA and BN = 16 .. 64
 //                          rows of A the other, so that a row of activations costs a column, not 1/128
-//                          of a tile, and what is streamed - the weights - fills whole tiles. K can be
-//                          split over a cluster whose CTAs add their partial tiles through distributed
-//                          shared memory, in split order.
+//                          of a tile. A thread then needs BN row scales per block, each read by all
+//                          lanes: 512 BN bytes per warp, four cycles per row at 128 bytes per cycle, which
+//                          at 128 rows took longer than everything else (0.75 us per block).
+//                          kWide = true: 128 rows of A on the 128-row side, one scale per thread.
 //   fp8_pair_kernel        many rows: 256 x 256 tiles on CTA pairs (cta_group::2).
 // All waits are bounded (ptx::mbar_wait) and reported through the device error word.
 #pragma once
+
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -61,6 +66,16 @@ struct Fp8Params {
 __device__ __forceinline__ void fp8_group_tables(const Fp8Params& p, int tile_rows, int* s_cu_tiles, int* s_row0,
                                                  int* s_rows) {
   const int G = p.num_groups;
+  if (p.seqlens == nullptr) {   // one group of all rows
+    if (threadIdx.x == 0) {
+      s_rows[0] = p.total_rows;
+      s_row0[0] = 0;
+      s_cu_tiles[0] = 0;
+      s_cu_tiles[1] = (p.total_rows + tile_rows - 1) / tile_rows;
+    }
+    __syncthreads();
+    return;
+  }
   for (int g = threadIdx.x; g < G; g += blockDim.x) {
     int row0 = p.cu_seqlens ? p.cu_seqlens[g] : 0;
     int rows = p.seqlens ? p.seqlens[g] : p.total_rows;
@@ -90,35 +105,11 @@ __device__ __forceinline__ void fp8_group_tables(const Fp8Params& p, int tile_ro
   __syncthreads();
 }
 
-// Starts the copies of one panel of scales into shared memory, [block][stride] floats: the scales of
-// `count` blocks of K from b0 on for ROWS rows, of which the first `valid` exist (the others become
-// zeros), and behind them those of TILES column tiles of B. Rows are kb floats apart in memory and of
-// any alignment, so the copies are 4 bytes each; eight neighbouring lanes take a row's eight blocks, which
-// is one sector (with a row per lane every copy was a sector of its own, and the eight blocks of a panel
-// fetched each of them again: the loader could not keep up with the MMAs).
-template <int ROWS, int TILES>
-__device__ __forceinline__ void fp8_load_scales(uint32_t dst, int stride, const float* a_scale, long long row, int valid, int kb,
-                                                int b0, int count, const float* b_scale, int tiles_left, int lane) {
-  const int j = lane & 7;
-  const bool block_in = j < count;
-  const float* src = a_scale + (row + (lane >> 3)) * kb + b0 + j;
-  const uint32_t to = dst + static_cast<uint32_t>(j * stride + (lane >> 3)) * 4;
-#pragma unroll 8
-  for (int r = 0; r < ROWS; r += 4) {
-    const bool in = r + (lane >> 3) < valid;
-    if (block_in) ptx::cp_async_4(to + 4 * r, in ? src + static_cast<long long>(r) * kb : a_scale, in);
-  }
-  const int tile = lane >> 3;
-  if (tile < TILES && block_in) {
-    const bool in = tile < tiles_left;
-    ptx::cp_async_4(dst + static_cast<uint32_t>(j * stride + ROWS + tile) * 4, in ? b_scale + static_cast<long long>(tile) * kb + b0 + j : b_scale, in);
-  }
-}
-
 // One output value, rounded once from FP32.
-__device__ __forceinline__ void fp8_store(void* out, int type, long long at, float v) {
-  if (type == kOutF16) static_cast<__half*>(out)[at] = __float2half_rn(v);
-  else if (type == kOutBf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+template <int kType>
+__device__ __forceinline__ void fp8_store(void* out, long long at, float v) {
+  if constexpr (kType == kOutF16) static_cast<__half*>(out)[at] = __float2half_rn(v);
+  else if constexpr (kType == kOutBf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
   else static_cast<float*>(out)[at] = v;
 }
 
@@ -128,19 +119,40 @@ __device__ __forceinline__ uint32_t fp8_pack2(int type, float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&b);
 }
 
+// Eight consecutive values, 16-byte aligned.
+template <int kType, typename Value>
+__device__ __forceinline__ void fp8_store8(void* out, long long at, Value value) {
+  if constexpr (kType == kOutF32) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+    dst[0] = make_float4(value(0), value(1), value(2), value(3));
+    dst[1] = make_float4(value(4), value(5), value(6), value(7));
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) =
+        make_uint4(fp8_pack2(kType, value(0), value(1)), fp8_pack2(kType, value(2), value(3)),
+                   fp8_pack2(kType, value(4), value(5)), fp8_pack2(kType, value(6), value(7)));
+  }
+}
+
 // --------------------------------------------------------------------- few rows
 
-template <int BN>
+template <int BN, bool kWide>
 struct Fp8SkinnyCfg {
-  static_assert(BN == 16 || BN == 32 || BN == 64 || BN == 128, "tile of 16 to 128 rows of A");
-  static constexpr int kThreads = 256;        // loaders of B, A and the scales, MMA issuer, four promotion warps
+  static_assert(kWide ? BN == 128 : BN == 16 || BN == 32 || BN == 64, "unsupported tile");
+  static constexpr int kTileM = kWide ? 128 : BN;          // rows of A per tile
+  static constexpr int kTileN = kWide ? BN : 128;          // rows of B (output columns) per tile
+  // promotion: a warp per quarter of tensor memory's lanes and, from 32 rows on, per half of the columns
+  static constexpr int kHalves = BN >= 32 ? 2 : 1;
+  static constexpr int kPromoters = 4 * kHalves;
+  static constexpr int kCols = BN / kHalves;               // accumulators of a promotion thread
+  static constexpr int kThreads = 128 + 32 * kPromoters;   // loaders of B and A, MMA issuer, (idle), promotion
+  static constexpr int kScales = kTileM * kFp8Panel / (32 * kPromoters);   // scales of a panel per promotion thread
   static constexpr int kBuffers = 4;          // block sums in tensor memory
   static constexpr int kTmemCols = kBuffers * BN < 32 ? 32 : kBuffers * BN;
-  static constexpr int kWBytes = 128 * kFp8BlockK;
-  static constexpr int kXBytes = BN * kFp8BlockK;
-  static constexpr int kStageBytes = kWBytes + kXBytes;
+  static constexpr int kWideBytes = 128 * kFp8BlockK;      // operand on the 128-row side of the MMA
+  static constexpr int kNarrowBytes = BN * kFp8BlockK;
+  static constexpr int kStageBytes = kWideBytes + kNarrowBytes;
   static constexpr int kMaxStages = 12;
-  static constexpr int kSlotFloats = BN + 4;  // row scales of one block, then the scale of the weights' tile (multiple of 4)
+  static constexpr int kSlotFloats = kTileM + 4;           // scales of one block, padded against bank conflicts
   static constexpr int kRedBytes = 128 * BN * 4;
   static constexpr int fixed_bytes(int groups, int splits) {
     return 1024 + 512 + kFp8Panels * kFp8Panel * kSlotFloats * 4 + 3 * (groups + 1) * 4 + (splits > 1 ? kRedBytes : 0);
@@ -152,15 +164,15 @@ struct Fp8SkinnyCfg {
   static constexpr int smem_bytes(int groups, int splits) {
     return fixed_bytes(groups, splits) + stages_for(groups, splits) * kStageBytes;
   }
-  static_assert(stages_for(kMaxGroups, 2) >= 4, "pipeline too shallow");
+  static_assert(stages_for(kMaxGroups, 2) >= 4 && stages_for(kMaxGroups, 2) * kStageBytes >= kRedBytes, "ring too small");
 };
 
-template <int BN>
-__global__ void __launch_bounds__(256, 1)
+template <int BN, bool kWide>
+__global__ void __launch_bounds__(Fp8SkinnyCfg<BN, kWide>::kThreads, 1)
 fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                   const Fp8Params p) {
-  using Cfg = Fp8SkinnyCfg<BN>;
-  constexpr int kLoadW = 0, kMma = 1, kLoadX = 2, kLoadS = 3, kFirstPromoter = 4;
+  using Cfg = Fp8SkinnyCfg<BN, kWide>;
+  constexpr int kLoadWide = 0, kMma = 1, kLoadNarrow = 2, kFirstPromoter = 4;
   const int kStages = p.num_stages;
   const int splits = p.splits;
   const int kb = (p.k + kFp8BlockK - 1) / kFp8BlockK;
@@ -173,10 +185,10 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   const uint32_t empty_u32 = full_u32 + 8 * Cfg::kMaxStages;           // ... have been read by the MMAs
   const uint32_t sum_full_u32 = empty_u32 + 8 * Cfg::kMaxStages;       // a block's sums are in tensor memory
   const uint32_t sum_empty_u32 = sum_full_u32 + 8 * Cfg::kBuffers;     // ... have been read
-  const uint32_t sc_full_u32 = sum_empty_u32 + 8 * Cfg::kBuffers;      // a block's scales are in their slot
-  const uint32_t sc_empty_u32 = sc_full_u32 + 8 * kFp8Panels;
-  const uint32_t red_full_u32 = sc_empty_u32 + 8 * kFp8Panels;     // every CTA's part of this CTA's columns
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kMaxStages + 2 * Cfg::kBuffers + 2 * kFp8Panels + 1);
+  const uint32_t sc_full_u32 = sum_empty_u32 + 8 * Cfg::kBuffers;      // a panel of scales is in shared memory
+  const uint32_t part_full_u32 = sc_full_u32 + 8 * kFp8Panels;         // this CTA's partial tile is in its ring
+  const uint32_t red_full_u32 = part_full_u32 + 8;                     // every CTA's part of this CTA's rows
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kMaxStages + 2 * Cfg::kBuffers + kFp8Panels + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
   float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);
   int* s_cu_tiles = reinterpret_cast<int*>(slots + kFp8Panels * kFp8Panel * Cfg::kSlotFloats);
@@ -186,11 +198,12 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int rank = splits > 1 ? static_cast<int>(ptx::cluster_cta_rank()) : 0;
+  const bool one_group = p.seqlens == nullptr;
 
   if (warp == 0) {
     if (lane == 0) {
       *abort_flag = 0;
-      ptx::prefetch_tensormap(&tmap_w);
+      ptx::prefetch_tensormap(kWide ? &tmap_x : &tmap_w);
     }
     for (int s = lane; s < kStages; s += 32) {
       ptx::mbar_init(full_u32 + 8 * s, 2);
@@ -198,28 +211,41 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     }
     if (lane < Cfg::kBuffers) {
       ptx::mbar_init(sum_full_u32 + 8 * lane, 1);
-      ptx::mbar_init(sum_empty_u32 + 8 * lane, 4);
+      ptx::mbar_init(sum_empty_u32 + 8 * lane, Cfg::kPromoters);
     }
-    if (lane < kFp8Panels) {
-      ptx::mbar_init(sc_full_u32 + 8 * lane, 32);
-      ptx::mbar_init(sc_empty_u32 + 8 * lane, 4);
-    }
+    if (lane < kFp8Panels) ptx::mbar_init(sc_full_u32 + 8 * lane, Cfg::kPromoters);
+    if (lane == 30) ptx::mbar_init(part_full_u32, Cfg::kPromoters);
     if (lane == 31) ptx::mbar_init(red_full_u32, 1);
+    if (one_group && lane == 0) {
+      s_rows[0] = p.total_rows;
+      s_row0[0] = 0;
+      s_cu_tiles[0] = 0;
+      s_cu_tiles[1] = (p.total_rows + Cfg::kTileM - 1) / Cfg::kTileM;
+    }
     __syncwarp();
     if (lane == 0) ptx::fence_barrier_init();
   } else if (warp == kMma) {
     ptx::tmem_alloc<1>(ptx::smem_u32(tmem_holder), Cfg::kTmemCols);
     ptx::tmem_relinquish<1>();
-  } else if (warp == kLoadX && lane == 0) {
-    ptx::prefetch_tensormap(&tmap_x);
+  } else if (warp == kLoadNarrow && lane == 0) {
+    ptx::prefetch_tensormap(kWide ? &tmap_w : &tmap_x);
   }
   ptx::tc_fence_before_sync();
-  fp8_group_tables(p, BN, s_cu_tiles, s_row0, s_rows);
+  if (one_group) {
+    // the loaders need the barriers only, and start before tensor memory has been allocated
+    if (warp == kLoadWide || warp == kLoadNarrow) {
+      ptx::named_barrier_sync(3, 64);
+      ptx::named_barrier_arrive(4, Cfg::kThreads);
+    } else {
+      ptx::named_barrier_sync(4, Cfg::kThreads);
+    }
+  } else {
+    fp8_group_tables(p, Cfg::kTileM, s_cu_tiles, s_row0, s_rows);
+  }
   if (splits > 1) ptx::cluster_arrive_relaxed();
   ptx::tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_holder;
 
-  const int n_tiles = (p.n + 127) / 128;
+  const int n_tiles = (p.n + Cfg::kTileN - 1) / Cfg::kTileN;
   const int total_mt = s_cu_tiles[p.num_groups];
   const int total_tasks = total_mt * n_tiles;
   // a cluster takes one task, a CTA of an unsplit launch as many as come its way
@@ -229,48 +255,30 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   const uint32_t stage_u32 = ptx::smem_u32(smem);
   bool met = false;             // this warp has waited for the cluster's set-up
 
-  if (warp == kLoadW || warp == kLoadX) {
-    const bool weights = warp == kLoadW;
-    const uint32_t bytes = weights ? Cfg::kWBytes : Cfg::kXBytes;
+  if (warp == kLoadWide || warp == kLoadNarrow) {
+    const bool wide = warp == kLoadWide, rows_of_a = wide == kWide;
+    const uint32_t bytes = wide ? Cfg::kWideBytes : Cfg::kNarrowBytes;
+    const CUtensorMap* tmap = rows_of_a ? &tmap_x : &tmap_w;
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true, withhold = weights && p.withhold_first_arrival != 0 && blockIdx.x == 0;
+    bool ok = true, withhold = wide && p.withhold_first_arrival != 0 && blockIdx.x == 0;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
       const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
-      const int row = weights ? t.g * p.n + t.nt * 128 : s_row0[t.g] + t.mt * BN;
+      const int row = rows_of_a ? s_row0[t.g] + t.mt * Cfg::kTileM : t.g * p.n + t.nt * Cfg::kTileN;
       for (int b = b_begin; b < b_end; ++b) {
         if (!ptx::mbar_wait(empty_u32 + 8 * stage, phase ^ 1, abort_flag, kWaitEmpty, p.wait_limit)) { ok = false; break; }
         if (ptx::elect_one()) {
           const uint32_t bar = full_u32 + 8 * stage;
           if (withhold) withhold = false;
           else ptx::mbar_arrive_expect_tx(bar, bytes);
-          ptx::tma_load_2d(stage_u32 + stage * Cfg::kStageBytes + (weights ? 0 : Cfg::kWBytes), weights ? &tmap_w : &tmap_x,
-                           bar, b * kFp8BlockK, row);
+          ptx::tma_load_2d(stage_u32 + stage * Cfg::kStageBytes + (wide ? 0 : Cfg::kWideBytes), tmap, bar, b * kFp8BlockK, row);
         }
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
     __syncwarp();
-  } else if (warp == kLoadS) {
-    int panel = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int task = first_task; task < total_tasks && ok; task += task_step) {
-      const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
-      const int row = s_row0[t.g] + t.mt * BN;
-      const int valid = min(BN, s_rows[t.g] - t.mt * BN);
-      const float* sb = p.b_scale + (static_cast<long long>(t.g) * n_tiles + t.nt) * kb;
-      for (int b0 = b_begin; b0 < b_end; b0 += kFp8Panel) {
-        if (!ptx::mbar_wait(sc_empty_u32 + 8 * panel, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
-        fp8_load_scales<BN, 1>(ptx::smem_u32(slots + panel * kFp8Panel * Cfg::kSlotFloats), Cfg::kSlotFloats, p.a_scale, row, valid,
-                               kb, b0, b_end - b0, sb, 1, lane);
-        ptx::cp_async_mbar_arrive(sc_full_u32 + 8 * panel);
-        if (++panel == kFp8Panels) { panel = 0; phase ^= 1; }
-      }
-    }
-    ptx::cp_async_wait_all();
-    __syncwarp();
   } else if (warp == kMma) {
+    const uint32_t tmem_base = *tmem_holder;
     constexpr uint32_t idesc = ptx::make_idesc_e4m3(128, BN);
     const uint32_t lo0 = ptx::kmajor_sw128_desc_lo(stage_u32);
     int stage = 0, buf = 0;
@@ -282,11 +290,11 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
             !ptx::mbar_wait(full_u32 + 8 * stage, phase, abort_flag, kWaitFull, p.wait_limit)) { ok = false; break; }
         ptx::tc_fence_after_sync();
         if (ptx::elect_one()) {
-          const uint32_t w_lo = lo0 + stage * (Cfg::kStageBytes >> 4);
-          const uint32_t x_lo = w_lo + (Cfg::kWBytes >> 4);
+          const uint32_t wide_lo = lo0 + stage * (Cfg::kStageBytes >> 4);
+          const uint32_t narrow_lo = wide_lo + (Cfg::kWideBytes >> 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j)      // 32 values of K = 32 bytes = 2 units of the address field
-            ptx::tc_mma_e4m3<1>(tmem_base + buf * BN, w_lo + 2 * j, x_lo + 2 * j, ptx::kKmajorSw128DescHi, idesc, j > 0 ? 1u : 0u);
+            ptx::tc_mma_e4m3<1>(tmem_base + buf * BN, wide_lo + 2 * j, narrow_lo + 2 * j, ptx::kKmajorSw128DescHi, idesc, j > 0 ? 1u : 0u);
           ptx::tc_commit<1>(empty_u32 + 8 * stage);
           ptx::tc_commit<1>(sum_full_u32 + 8 * buf);
         }
@@ -296,103 +304,190 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       }
     }
     __syncwarp();
-  } else {
-    // ------------------------------ promotion: lane = row of B (output column), register = row of A
+  } else if (warp >= kFirstPromoter) {
+    // ------------ promotion. kWide: lane = row of A, register = output column; else the other way round
     const int q = warp & 3;
-    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-    constexpr int kChunk = BN < 32 ? BN : 32;
+    const int col_first = (warp - kFirstPromoter) / 4 * Cfg::kCols;
+    const uint32_t lane_addr = *tmem_holder + (static_cast<uint32_t>(q * 32) << 16) + col_first;
+    const int tile_row = q * 32 + lane;
+    const int tid = static_cast<int>(threadIdx.x) - 32 * kFirstPromoter;
+    // The promotion threads fetch the scales themselves, a panel of eight blocks ahead: into registers
+    // while the last panel is used, then, each row scale times that of the weights' tile, into shared memory
+    // as [block][rows of A]. Eight neighbouring lanes take the eight blocks of a row, which is one sector.
+    // (A loader warp with asynchronous copies had the first panel ready 2000 cycles after the operands.)
+    float next_scale[Cfg::kScales], next_w_scale = 0.0f;
+    auto fetch_scales = [&](int task, int b0) {
+      const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
+      const int left = s_rows[t.g] - t.mt * Cfg::kTileM;
+      const int j = tid & 7;
+      const float* src = p.a_scale + static_cast<long long>(s_row0[t.g] + t.mt * Cfg::kTileM) * kb + b0 + j;
+      const long long tile = static_cast<long long>(t.g) * ((p.n + 127) / 128) + t.nt * Cfg::kTileN / 128;
+      next_w_scale = b0 + j < b_end ? __ldg(p.b_scale + tile * kb + b0 + j) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < Cfg::kScales; ++i) {
+        const int r = (tid >> 3) + i * (4 * Cfg::kPromoters);
+        next_scale[i] = r < left && b0 + j < b_end ? __ldg(src + static_cast<long long>(r) * kb) : 0.0f;
+      }
+    };
     int buf = 0, panel = 0;
     uint32_t buf_phase = 0, panel_phase = 0;
     bool ok = true;
+    if (first_task < total_tasks && b_begin < b_end) fetch_scales(first_task, b_begin);
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
       const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
-      const int valid = min(BN, s_rows[t.g] - t.mt * BN);
-      float acc[BN];
+      // rows of A and output columns of the tile that exist; `valid` are those the registers run over
+      const int rows_in = min(Cfg::kTileM, s_rows[t.g] - t.mt * Cfg::kTileM), cols_in = min(Cfg::kTileN, p.n - t.nt * Cfg::kTileN);
+      const int valid = kWide ? cols_in : rows_in;
+      float acc[Cfg::kCols];
 #pragma unroll
-      for (int c = 0; c < BN; ++c) acc[c] = 0.0f;
-      for (int b = b_begin; b < b_end; ++b) {
-        const int in_panel = (b - b_begin) & (kFp8Panel - 1);
-        if ((in_panel == 0 && !ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) ||
-            !ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
-        ptx::tc_fence_after_sync();
-        const float* sc = slots + (panel * kFp8Panel + in_panel) * Cfg::kSlotFloats;
-        const float sb = sc[BN];
+      for (int c = 0; c < Cfg::kCols; ++c) acc[c] = 0;
+      const float* sc = nullptr;
+      for (int b = b_begin; b < b_end; ++b, sc += Cfg::kSlotFloats) {
+        if (((b - b_begin) & (kFp8Panel - 1)) == 0) {
+          // (a warp reaches this panel's buffer again only after all have used it: each arrives here in between)
+          float* to = slots + panel * kFp8Panel * Cfg::kSlotFloats;
 #pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += kChunk) {
-          uint32_t v[kChunk];
-          ptx::tmem_ld_cols<kChunk>(lane_addr + buf * BN + c0, v);
-          ptx::tmem_ld_wait_regs<kChunk>(v);
-#pragma unroll
-          for (int c = 0; c < kChunk; c += 4) {
-            const float4 sa = *reinterpret_cast<const float4*>(sc + c0 + c);
-            acc[c0 + c] = fmaf(__uint_as_float(v[c]), sa.x * sb, acc[c0 + c]);
-            acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), sa.y * sb, acc[c0 + c + 1]);
-            acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), sa.z * sb, acc[c0 + c + 2]);
-            acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), sa.w * sb, acc[c0 + c + 3]);
-          }
+          for (int i = 0; i < Cfg::kScales; ++i) to[(tid & 7) * Cfg::kSlotFloats + (tid >> 3) + i * (4 * Cfg::kPromoters)] = next_scale[i] * next_w_scale;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(sc_full_u32 + 8 * panel);
+          if (b + kFp8Panel < b_end) fetch_scales(task, b + kFp8Panel);
+          else if (task + task_step < total_tasks) fetch_scales(task + task_step, b_begin);
+          if (!ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
+          sc = to;
+          if (++panel == kFp8Panels) { panel = 0; panel_phase ^= 1; }
         }
+        if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
+        ptx::tc_fence_after_sync();
+        // all columns first, one wait: the reads of the scales then follow each other without it
+        constexpr int kStep = Cfg::kCols < 32 ? 16 : 32;
+        uint32_t v[Cfg::kCols / kStep][kStep];
+#pragma unroll
+        for (int c = 0; c < Cfg::kCols / kStep; ++c) ptx::tmem_ld_cols<kStep>(lane_addr + buf * BN + c * kStep, v[c]);
+#pragma unroll
+        for (int c = 0; c < Cfg::kCols / kStep; ++c) ptx::tmem_ld_wait_regs<kStep>(v[c]);
         ptx::tc_fence_before_sync();
         __syncwarp();
-        const bool panel_done = in_panel == kFp8Panel - 1 || b + 1 == b_end;
-        if (lane == 0) {
-          ptx::mbar_arrive(sum_empty_u32 + 8 * buf);
-          if (panel_done) ptx::mbar_arrive(sc_empty_u32 + 8 * panel);
+        if (lane == 0) ptx::mbar_arrive(sum_empty_u32 + 8 * buf);
+        if constexpr (kWide) {
+          const float by = sc[tile_row];
+#pragma unroll
+          for (int c = 0; c < Cfg::kCols; ++c) acc[c] = fmaf(__uint_as_float(v[c / kStep][c % kStep]), by, acc[c]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < Cfg::kCols; c += 4) {
+            const float4 sa = *reinterpret_cast<const float4*>(sc + col_first + c);
+            const uint32_t* x = &v[c / kStep][c % kStep];
+            acc[c] = fmaf(__uint_as_float(x[0]), sa.x, acc[c]);
+            acc[c + 1] = fmaf(__uint_as_float(x[1]), sa.y, acc[c + 1]);
+            acc[c + 2] = fmaf(__uint_as_float(x[2]), sa.z, acc[c + 2]);
+            acc[c + 3] = fmaf(__uint_as_float(x[3]), sa.w, acc[c + 3]);
+          }
         }
         if (++buf == Cfg::kBuffers) { buf = 0; buf_phase ^= 1; }
-        if (panel_done && ++panel == kFp8Panels) { panel = 0; panel_phase ^= 1; }
       }
       if (!ok) break;
-      const int tile_row = q * 32 + lane;
-      const int col = t.nt * 128 + tile_row;                      // output column
-      const long long out0 = (static_cast<long long>(s_row0[t.g]) + t.mt * BN) * p.n + col;
+      auto value = [&](int c) { return acc[c]; };
+      const long long out0 = (static_cast<long long>(s_row0[t.g]) + t.mt * Cfg::kTileM) * p.n + t.nt * Cfg::kTileN;
       if (splits == 1) {
-        if (col < p.n) {
+        auto store_all = [&](auto type) {
+          constexpr int kType = decltype(type)::value;
+          if constexpr (kWide) {
+            if (tile_row < rows_in) {
+              const long long at = out0 + static_cast<long long>(tile_row) * p.n + col_first;
 #pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (c < valid) fp8_store(p.out, p.out_type, out0 + static_cast<long long>(c) * p.n, acc[c]);
-        }
+              for (int c = 0; c < Cfg::kCols; c += 8)            // n is a multiple of 8
+                if (col_first + c < valid) fp8_store8<kType>(p.out, at + c, [&](int j) { return value(c + j); });
+            }
+          } else if (tile_row < cols_in) {
+#pragma unroll
+            for (int c = 0; c < Cfg::kCols; ++c)
+              if (col_first + c < valid)
+                fp8_store<kType>(p.out, out0 + static_cast<long long>(col_first + c) * p.n + tile_row, value(c));
+          }
+        };
+        if (p.out_type == kOutF16) store_all(std::integral_constant<int, kOutF16>());
+        else if (p.out_type == kOutBf16) store_all(std::integral_constant<int, kOutBf16>());
+        else store_all(std::integral_constant<int, kOutF32>());
       } else {
-        // CTA d of the cluster finishes rows [d w, (d + 1) w) of the tile: everybody stores its part
-        // into slot `rank` of that CTA's buffer, [slot][row][128 columns], counted in bytes there.
-        const int w = (valid + splits - 1) / splits;
+        // CTA d of the cluster finishes register columns [d w, (d + 1) w) of the tile. Everybody lays its
+        // partial tile into its (now idle) operand ring, [register column][128 lanes], and copies slice d into CTA d's buffer,
+        // one bulk copy each, counted in bytes on the receiver's barrier. (Asynchronous stores of single
+        // words took longer than the product: 64 x 7168 x 2048 14.4 us unsplit, 18.5 split in two.)
+        const int w = kWide ? BN / splits : (valid + splits - 1) / splits;
         const int mine = max(0, min(w, valid - rank * w));
-        if (warp == kFirstPromoter && lane == 0 && mine > 0)
-          ptx::mbar_arrive_expect_tx(red_full_u32, static_cast<uint32_t>(splits * mine * 128 * 4));
+        const bool first = warp == kFirstPromoter && lane == 0;
+        if (first && mine > 0) ptx::mbar_arrive_expect_tx(red_full_u32, static_cast<uint32_t>((splits - 1) * mine * 512));
+#pragma unroll
+        for (int c = 0; c < Cfg::kCols; ++c)
+          if (col_first + c < valid) reinterpret_cast<float*>(smem)[(col_first + c) * 128 + tile_row] = value(c);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(part_full_u32);
         ptx::cluster_wait();                                       // every CTA has its barriers
         met = true;
+        if (!ptx::mbar_wait(part_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
         const uint32_t red_u32 = ptx::smem_u32(red);
-        int d = 0, at = 0;
-        uint32_t base = ptx::map_to_cta(red_u32, 0), bar = ptx::map_to_cta(red_full_u32, 0);
-        int rows_d = min(w, valid);
-#pragma unroll
-        for (int c = 0; c < BN; ++c) {
-          if (c < valid) {
-            if (at == w) {
-              ++d;
-              at = 0;
-              base = ptx::map_to_cta(red_u32, d);
-              bar = ptx::map_to_cta(red_full_u32, d);
-              rows_d = min(w, valid - d * w);
-            }
-            ptx::st_async_b32(base + static_cast<uint32_t>(((rank * rows_d + at) * 128 + tile_row) * 4), __float_as_uint(acc[c]), bar);
-            ++at;
+        if (first) {
+          for (int d = 0; d < splits; ++d) {
+            const int rows_d = min(w, valid - d * w);
+            if (d == rank || rows_d <= 0) continue;
+            ptx::bulk_copy_to_cta(ptx::map_to_cta(red_u32 + static_cast<uint32_t>(rank * rows_d * 512), d),
+                                  stage_u32 + static_cast<uint32_t>(d * w * 512), static_cast<uint32_t>(rows_d * 512),
+                                  ptx::map_to_cta(red_full_u32, d));
           }
         }
         if (mine > 0) {
           if (!ptx::mbar_wait_cluster(red_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
-          const float* part = reinterpret_cast<const float*>(red);
-          for (int i = 0; i < mine; ++i) {
-            float sum = part[i * 128 + tile_row];
-            for (int s = 1; s < splits; ++s) sum = __fadd_rn(sum, part[(s * mine + i) * 128 + tile_row]);
-            if (col < p.n) fp8_store(p.out, p.out_type, out0 + static_cast<long long>(rank * w + i) * p.n, sum);
-          }
+          // partial sums in split order, two columns per thread
+          auto reduce = [&](auto count) {
+            constexpr int kSplits = decltype(count)::value;
+            // sum of the partial values at (register column i, 128-side index l .. l + 1), in split order
+            auto sum2 = [&](int i, int l) {
+              float2 v[kSplits];
+#pragma unroll
+              for (int s = 0; s < kSplits; ++s) {
+                const float* part = s == rank ? reinterpret_cast<const float*>(smem) + (rank * w + i) * 128
+                                              : reinterpret_cast<const float*>(red) + (s * mine + i) * 128;
+                v[s] = *reinterpret_cast<const float2*>(part + l);
+              }
+#pragma unroll
+              for (int s = 1; s < kSplits; ++s) {
+                v[0].x = __fadd_rn(v[0].x, v[s].x);
+                v[0].y = __fadd_rn(v[0].y, v[s].y);
+              }
+              return v[0];
+            };
+            auto store2 = [&](long long at, float2 v) {              // at is even
+              if (p.out_type == kOutF32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at) = v;
+              else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at) = fp8_pack2(p.out_type, v.x, v.y);
+            };
+            if constexpr (kWide) {
+              // two rows by two columns per thread and step; w is even, and so is the slice's end
+              for (int x = tid; x < (mine >> 1) * 64; x += 32 * Cfg::kPromoters) {
+                const int i = 2 * (x >> 6), l = 2 * (x & 63);
+                const float2 a = sum2(i, l), b = sum2(i + 1, l);
+                const long long at = out0 + static_cast<long long>(l) * p.n + rank * w + i;
+                if (l < rows_in) store2(at, make_float2(a.x, b.x));
+                if (l + 1 < rows_in) store2(at + p.n, make_float2(a.y, b.y));
+              }
+            } else {
+              for (int x = tid; x < mine * 64; x += 32 * Cfg::kPromoters) {
+                const int i = x >> 6, l = 2 * (x & 63);
+                const float2 v = sum2(i, l);
+                if (l < cols_in) store2(out0 + static_cast<long long>(rank * w + i) * p.n + l, v);
+              }
+            }
+          };
+          if (splits == 2) reduce(std::integral_constant<int, 2>());
+          else if (splits == 4) reduce(std::integral_constant<int, 4>());
+          else reduce(std::integral_constant<int, 8>());
         }
       }
     }
     __syncwarp();
   }
 
-  // ---- teardown
+  // ---- teardown (a CTA of a cluster must outlive its copies: their receivers arrive after having got them)
   if (splits > 1 && !met) ptx::cluster_wait();     // every thread waits once for the arrival at set-up
   __syncthreads();
   const int aborted = *abort_flag;
@@ -405,7 +500,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   }
   if (warp == kMma) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc<1>(tmem_base, Cfg::kTmemCols);
+    ptx::tmem_dealloc<1>(*tmem_holder, Cfg::kTmemCols);
   }
 }
 
@@ -415,7 +510,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 // MMAs read both halves, and each CTA's tensor memory receives 128 rows x 256 columns of a block's
 // sums. Two such buffers fill the 512 columns of tensor memory. 128 accumulators per thread in eight
 // promotion warps need more registers than an even share (65536 / 384 = 168): the other four warps
-// give theirs up (72 + 2 x 216 = 504 = 3 x 168).
+// give theirs up (104 + 2 x 200 = 504 = 3 x 168; 56 / 224 to 104 / 200 differ by what the compiler spills: measured).
 struct Fp8PairCfg {
   static constexpr int kThreads = 384;
   static constexpr int kBuffers = 2;
@@ -513,7 +608,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
   // (each share is set where its code begins: after a join the compiler would hold both to the smaller)
   if (warp < kFirstPromoter) {
-  ptx::setmaxnreg_dec<72>();
+  ptx::setmaxnreg_dec<104>();
   if (warp == kLoadA || warp == kLoadB) {
     const bool is_a = warp == kLoadA;
     const CUtensorMap* tmap = is_a ? &tmap_a : &tmap_b;
@@ -605,7 +700,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     __syncwarp();
   }
   } else {
-    ptx::setmaxnreg_inc<216>();
+    ptx::setmaxnreg_inc<200>();
     // ------------------ promotion: lane = row of the tile, registers = 128 columns (one scale tile of B)
     const int q = warp & 3;
     const int half = (warp - kFirstPromoter) >> 2;
@@ -618,9 +713,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     bool ok = true;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
       const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
-      uint64_t acc[64];                      // column pairs, as the packed FMA takes them
+      float acc[128];
 #pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = 0;
+      for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
       float4 s4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int b = 0; b < kb; ++b) {
         if ((b & (Cfg::kPanel - 1)) == 0) {
@@ -632,7 +727,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           if (lane == 0) ptx::mbar_arrive(sc_empty_u32 + 8 * panel);
           if (++panel == Cfg::kPanels) { panel = 0; panel_phase ^= 1; }
         }
-        const uint64_t s = ptx::pack_f32x2(__float_as_uint(s4.x), __float_as_uint(s4.x));
+        const float s = s4.x;
         s4 = make_float4(s4.y, s4.z, s4.w, s4.x);
         if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
         ptx::tc_fence_after_sync();
@@ -651,11 +746,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             }
           }
 #pragma unroll
-          for (int c = 0; c < 8; ++c) ptx::fma_f32x2(acc[c0 * 8 + c], ptx::pack_f32x2(v[2 * c], v[2 * c + 1]), s);
+          for (int c = 0; c < 16; ++c) acc[c0 * 16 + c] = fmaf(__uint_as_float(v[c]), s, acc[c0 * 16 + c]);
         }
         if (++buf == Cfg::kBuffers) { buf = 0; buf_phase ^= 1; }
       }
-      auto value = [&](int c) { return __uint_as_float(static_cast<uint32_t>(c & 1 ? acc[c >> 1] >> 32 : acc[c >> 1])); };
+      auto value = [&](int c) { return acc[c]; };
       if (!ok) break;
       // ---- output: a slab of 32 valid rows leaves through the staging buffer and the store engine,
       // a ragged one by predicated stores
@@ -704,15 +799,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         for (int c = 0; c < 128; c += 8) {               // n is a multiple of 8
           const int col = col0 + c;
           if (col < p.n) {
-            if (elem == 4) {
-              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + col);
-              dst[0] = make_float4(value(c), value(c + 1), value(c + 2), value(c + 3));
-              dst[1] = make_float4(value(c + 4), value(c + 5), value(c + 6), value(c + 7));
-            } else {
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + col) =
-                  make_uint4(fp8_pack2(p.out_type, value(c), value(c + 1)), fp8_pack2(p.out_type, value(c + 2), value(c + 3)),
-                             fp8_pack2(p.out_type, value(c + 4), value(c + 5)), fp8_pack2(p.out_type, value(c + 6), value(c + 7)));
-            }
+            auto eight = [&](int j) { return value(c + j); };
+            if (p.out_type == kOutF32) fp8_store8<kOutF32>(p.out, at + col, eight);
+            else if (p.out_type == kOutF16) fp8_store8<kOutF16>(p.out, at + col, eight);
+            else fp8_store8<kOutBf16>(p.out, at + col, eight);
           }
         }
       }

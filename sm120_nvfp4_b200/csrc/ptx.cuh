@@ -415,6 +415,11 @@ __device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
   return r;
 }
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
@@ -513,10 +518,13 @@ __device__ __forceinline__ void st_async_v4(uint32_t addr, uint32_t a, uint32_t 
                : "memory");
 }
 
-// The same for 4 bytes.
-__device__ __forceinline__ void st_async_b32(uint32_t addr, uint32_t a, uint32_t bar_cluster_addr) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(a),
-               "r"(bar_cluster_addr)
+// Bulk copy from this CTA's shared memory into that of a CTA of the cluster (addresses and size multiples
+// of 16 bytes); the bytes count on the mbarrier `bar_cluster_addr`, which lies in the receiving CTA.
+__device__ __forceinline__ void bulk_copy_to_cta(uint32_t dst_cluster_addr, uint32_t src, uint32_t bytes,
+                                                 uint32_t bar_cluster_addr) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   dst_cluster_addr),
+               "r"(src), "r"(bytes), "r"(bar_cluster_addr)
                : "memory");
 }
 
