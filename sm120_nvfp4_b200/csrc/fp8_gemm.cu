@@ -135,24 +135,41 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
   return launch_status();
 }
 
-// Rows of A per tile: the smallest skinny tile that holds a group's rows, CTA pairs once there are
-// enough 256 x 256 tiles.
-int pick_fp8_tile(const Fp8Problem& q, const DeviceInfo& dev) {
-  const int rows = q.avg_rows;
-  if (rows <= 16) return 16;
-  if (rows <= 32) return 32;
-  if (rows <= 64) return 64;
-  const long long pairs = row_tiles(q, 256) * ((q.n + 255) / 256);
-  return rows > 128 && pairs * 2 >= dev.sm_count / 2 ? kPairTile : 128;
-}
-
-// CTAs per tile over K: as many as still fit the GPU at once and leave each at least two blocks of K.
+// CTAs per tile over K: as many as still fit the GPU at once and leave each enough blocks of K to pay for the
+// exchange of partial tiles, which grows with the tile (us, tile / splits; 24 x 1024 x 1024: 16/1 6.3,
+// 16/4 5.9; 64 x 7168 x 2048: 64/1 10.6, 64/2 10.3; 128 x 7168 x 2048: 128/1 12.8, 128/2 14.8;
+// 128 x 4096 x 7168: 128/1 29.5, 128/4 17.2).
 int pick_fp8_splits(const Fp8Problem& q, const DeviceInfo& dev, int tile) {
   const long long tasks = row_tiles(q, tile) * ((q.n + 127) / 128);
   const int kb = (q.k + kFp8BlockK - 1) / kFp8BlockK;
+  const int least = tile == 16 ? 2 : (tile == 128 ? 12 : 4);
   for (int s = 8; s >= 2; s /= 2)
-    if (tasks * s <= dev.sm_count && kb >= 2 * s) return s;
+    if (tasks * s <= dev.sm_count && kb >= least * s) return s;
   return 1;
+}
+
+// Rows of A per tile (512: 256 x 256 on CTA pairs).
+//   Groups: the tile that the average group fills to at most three quarters, since groups differ; every
+//   further tile of a group reads its weights again. 32 groups over 4096 x 7168, us for the average row
+//   counts 12 / 24 / 40 / 64 / 96 / 128: 16 rows 151 / 226 / - , 32 rows 148 / 157 / 218 / 320,
+//   64 rows 164 / 167 / 172 / 256 / 324, 128 rows 177 / 178 / 182 / 185 / 215 / 289, pairs - / - / 216 / 218 /
+//   220 / 219.
+//   One group: the smallest tile that holds all rows up to 64; then 128 rows where K is deep enough to be
+//   split (128 x 4096 x 7168: 17.2 us, 64 rows 17.7) or the tiles fit the GPU at once, 64 rows while even
+//   those do (128 x 7168 x 2048: 11.0 against 12.8), pairs beyond (384 x 7168 x 2048: 14.3 against 22.0).
+int pick_fp8_tile(const Fp8Problem& q, const DeviceInfo& dev) {
+  const int rows = q.avg_rows;
+  if (q.seqlens != nullptr) {
+    for (int tile = 16; tile <= 128; tile *= 2)
+      if (static_cast<long long>(rows) * 4 <= tile * 3) return tile;
+    return kPairTile;
+  }
+  for (int tile = 16; tile <= 64; tile *= 2)
+    if (rows <= tile) return tile;
+  const long long columns = (q.n + 127) / 128;
+  if (pick_fp8_splits(q, dev, 128) > 1) return 128;
+  if (row_tiles(q, 64) * columns <= dev.sm_count) return 64;
+  return row_tiles(q, 128) * columns <= dev.sm_count ? 128 : kPairTile;
 }
 
 int fp8_product(const Fp8Problem& q, const void* a_scale, const void* b_scale, void* out, int out_type, cudaStream_t stream) {

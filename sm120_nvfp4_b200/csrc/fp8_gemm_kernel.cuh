@@ -342,48 +342,88 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 #pragma unroll
       for (int c = 0; c < Cfg::kCols; ++c) acc[c] = 0;
       const float* sc = nullptr;
-      for (int b = b_begin; b < b_end; ++b, sc += Cfg::kSlotFloats) {
-        if (((b - b_begin) & (kFp8Panel - 1)) == 0) {
-          // (a warp reaches this panel's buffer again only after all have used it: each arrives here in between)
-          float* to = slots + panel * kFp8Panel * Cfg::kSlotFloats;
-#pragma unroll
-          for (int i = 0; i < Cfg::kScales; ++i) to[(tid & 7) * Cfg::kSlotFloats + (tid >> 3) + i * (4 * Cfg::kPromoters)] = next_scale[i] * next_w_scale;
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(sc_full_u32 + 8 * panel);
-          if (b + kFp8Panel < b_end) fetch_scales(task, b + kFp8Panel);
-          else if (task + task_step < total_tasks) fetch_scales(task + task_step, b_begin);
-          if (!ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
-          sc = to;
-          if (++panel == kFp8Panels) { panel = 0; panel_phase ^= 1; }
+      // Scales of block b, in shared memory from its panel's first block on. (A warp reaches a panel's buffer
+      // again only after all have used it: each arrives at the other panel's barrier in between.)
+      auto scales_for = [&](int b) {
+        if (((b - b_begin) & (kFp8Panel - 1)) != 0) {
+          sc += Cfg::kSlotFloats;
+          return true;
         }
-        if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
+        float* to = slots + panel * kFp8Panel * Cfg::kSlotFloats;
+#pragma unroll
+        for (int i = 0; i < Cfg::kScales; ++i) to[(tid & 7) * Cfg::kSlotFloats + (tid >> 3) + i * (4 * Cfg::kPromoters)] = next_scale[i] * next_w_scale;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(sc_full_u32 + 8 * panel);
+        if (b + kFp8Panel < b_end) fetch_scales(task, b + kFp8Panel);
+        else if (task + task_step < total_tasks) fetch_scales(task + task_step, b_begin);
+        if (!ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) return false;
+        sc = to;
+        if (++panel == kFp8Panels) { panel = 0; panel_phase ^= 1; }
+        return true;
+      };
+      auto sums_ready = [&] {
+        if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) return false;
         ptx::tc_fence_after_sync();
-        // all columns first, one wait: the reads of the scales then follow each other without it
-        constexpr int kStep = Cfg::kCols < 32 ? 16 : 32;
-        uint32_t v[Cfg::kCols / kStep][kStep];
-#pragma unroll
-        for (int c = 0; c < Cfg::kCols / kStep; ++c) ptx::tmem_ld_cols<kStep>(lane_addr + buf * BN + c * kStep, v[c]);
-#pragma unroll
-        for (int c = 0; c < Cfg::kCols / kStep; ++c) ptx::tmem_ld_wait_regs<kStep>(v[c]);
+        return true;
+      };
+      auto release_sums = [&] {
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(sum_empty_u32 + 8 * buf);
-        if constexpr (kWide) {
+        if (++buf == Cfg::kBuffers) { buf = 0; buf_phase ^= 1; }
+      };
+      if constexpr (kWide) {
+        // The loads run one step of 16 columns ahead of the additions, across blocks too: the first step of
+        // the next block is on its way while the last of this one is added. (Steps of 32 spill.)
+        constexpr int kSteps = Cfg::kCols / 16;
+        static_assert(kSteps % 2 == 0, "the first step of a block uses the first buffer");
+        uint32_t v[2][16];
+        if (b_begin < b_end) {
+          ok = sums_ready();
+          if (ok) ptx::tmem_ld_cols<16>(lane_addr + buf * BN, v[0]);
+        }
+        for (int b = b_begin; b < b_end && ok; ++b) {
+          ok = scales_for(b);
+          if (!ok) break;
           const float by = sc[tile_row];
 #pragma unroll
-          for (int c = 0; c < Cfg::kCols; ++c) acc[c] = fmaf(__uint_as_float(v[c / kStep][c % kStep]), by, acc[c]);
-        } else {
+          for (int step = 0; step < kSteps; ++step) {
+            ptx::tmem_ld_wait_regs<16>(v[step & 1]);
+            if (step + 1 < kSteps) {
+              ptx::tmem_ld_cols<16>(lane_addr + buf * BN + (step + 1) * 16, v[(step + 1) & 1]);
+            } else {
+              release_sums();
+              if (b + 1 < b_end) {
+                ok = sums_ready();
+                if (!ok) break;
+                ptx::tmem_ld_cols<16>(lane_addr + buf * BN, v[0]);
+              }
+            }
 #pragma unroll
-          for (int c = 0; c < Cfg::kCols; c += 4) {
-            const float4 sa = *reinterpret_cast<const float4*>(sc + col_first + c);
-            const uint32_t* x = &v[c / kStep][c % kStep];
-            acc[c] = fmaf(__uint_as_float(x[0]), sa.x, acc[c]);
-            acc[c + 1] = fmaf(__uint_as_float(x[1]), sa.y, acc[c + 1]);
-            acc[c + 2] = fmaf(__uint_as_float(x[2]), sa.z, acc[c + 2]);
-            acc[c + 3] = fmaf(__uint_as_float(x[3]), sa.w, acc[c + 3]);
+            for (int c = 0; c < 16; ++c) acc[step * 16 + c] = fmaf(__uint_as_float(v[step & 1][c]), by, acc[step * 16 + c]);
           }
         }
-        if (++buf == Cfg::kBuffers) { buf = 0; buf_phase ^= 1; }
+        ptx::tmem_ld_wait();                                       // nothing may stay in flight after a break
+      } else {
+        for (int b = b_begin; b < b_end; ++b) {
+          ok = scales_for(b) && sums_ready();
+          if (!ok) break;
+          // all columns first, one wait: the reads of the scales then follow each other without it
+          constexpr int kStep = Cfg::kCols < 32 ? 16 : 32;
+          static_assert(kStep == Cfg::kCols, "one load");
+          uint32_t v[kStep];
+          ptx::tmem_ld_cols<kStep>(lane_addr + buf * BN, v);
+          ptx::tmem_ld_wait_regs<kStep>(v);
+          release_sums();
+#pragma unroll
+          for (int c = 0; c < kStep; c += 4) {
+            const float4 sa = *reinterpret_cast<const float4*>(sc + col_first + c);
+            acc[c] = fmaf(__uint_as_float(v[c]), sa.x, acc[c]);
+            acc[c + 1] = fmaf(__uint_as_float(v[c + 1]), sa.y, acc[c + 1]);
+            acc[c + 2] = fmaf(__uint_as_float(v[c + 2]), sa.z, acc[c + 2]);
+            acc[c + 3] = fmaf(__uint_as_float(v[c + 3]), sa.w, acc[c + 3]);
+          }
+        }
       }
       if (!ok) break;
       auto value = [&](int c) { return acc[c]; };
@@ -462,13 +502,27 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
               else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at) = fp8_pack2(p.out_type, v.x, v.y);
             };
             if constexpr (kWide) {
-              // two rows by two columns per thread and step; w is even, and so is the slice's end
-              for (int x = tid; x < (mine >> 1) * 64; x += 32 * Cfg::kPromoters) {
-                const int i = 2 * (x >> 6), l = 2 * (x & 63);
-                const float2 a = sum2(i, l), b = sum2(i + 1, l);
-                const long long at = out0 + static_cast<long long>(l) * p.n + rank * w + i;
-                if (l < rows_in) store2(at, make_float2(a.x, b.x));
-                if (l + 1 < rows_in) store2(at + p.n, make_float2(a.y, b.y));
+              // eight columns of a row per thread: neighbouring lanes read neighbouring words, and store 16
+              // (32) bytes of their own row; w is a multiple of 8, so are the slices' ends
+              for (int x = tid; x < (mine >> 3) * 128; x += 32 * Cfg::kPromoters) {
+                const int i = 8 * (x >> 7), l = x & 127;
+                float sum[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+#pragma unroll
+                  for (int s = 0; s < kSplits; ++s) {
+                    const float* part = s == rank ? reinterpret_cast<const float*>(smem) + (rank * w + i + c) * 128
+                                                  : reinterpret_cast<const float*>(red) + (s * mine + i + c) * 128;
+                    sum[c] = s == 0 ? part[l] : __fadd_rn(sum[c], part[l]);
+                  }
+                }
+                if (l < rows_in) {
+                  const long long at = out0 + static_cast<long long>(l) * p.n + rank * w + i;
+                  auto eight = [&](int c) { return sum[c]; };
+                  if (p.out_type == kOutF32) fp8_store8<kOutF32>(p.out, at, eight);
+                  else if (p.out_type == kOutF16) fp8_store8<kOutF16>(p.out, at, eight);
+                  else fp8_store8<kOutBf16>(p.out, at, eight);
+                }
               }
             } else {
               for (int x = tid; x < mine * 64; x += 32 * Cfg::kPromoters) {
