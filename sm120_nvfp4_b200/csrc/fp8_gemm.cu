@@ -15,6 +15,7 @@ extern std::atomic<int> g_withhold_once;
 namespace {
 
 constexpr int kPairTile = 512;
+constexpr int kMaxRows = 0x7fffff00;
 
 std::atomic<int> g_fp8_tile{0};
 std::atomic<int> g_fp8_splits{0};
@@ -205,7 +206,8 @@ int fp8_product(const Fp8Problem& q, const void* a_scale, const void* b_scale, v
 }
 
 bool valid_fp8(int rows, int n, int k, int out_type) {
-  return rows >= 0 && n > 0 && k > 0 && (k % 16) == 0 && (n % 8) == 0 && out_type >= kOutF16 && out_type <= kOutBf16;
+  // (row coordinates of a tile that reaches past the end still have to fit 32 bits)
+  return rows >= 0 && rows <= kMaxRows && n > 0 && n <= kMaxRows && k > 0 && (k % 16) == 0 && (n % 8) == 0 && out_type >= kOutF16 && out_type <= kOutBf16;
 }
 
 }  // namespace
@@ -229,7 +231,7 @@ int b200_nvfp4_fp8_grouped_gemm(void* y, const void* x, const void* w, const voi
   using namespace b200;
   if (!valid_fp8(m, n, k, out_type) || num_group <= 0 || num_group > kMaxGroups || y == nullptr || x == nullptr ||
       w == nullptr || seqlens == nullptr || cu_seqlens == nullptr || x_scale == nullptr || w_scale == nullptr ||
-      !aligned16(y) || !aligned16(x) || !aligned16(w) || static_cast<long long>(num_group) * n > 0x7fffffffLL)
+      !aligned16(y) || !aligned16(x) || !aligned16(w) || static_cast<long long>(num_group) * n > kMaxRows)
     return B200_NVFP4_INVALID_ARGUMENT;
   const int avg = num_seq_per_group_avg > 0 ? num_seq_per_group_avg : (m + num_group - 1) / num_group;
   const Fp8Problem q{num_group, m, n, k, x, w, static_cast<const int*>(seqlens), static_cast<const int*>(cu_seqlens), avg};

@@ -228,7 +228,8 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         if (col < p.experts) {
           const Vec<float, V> x = *reinterpret_cast<const Vec<float, V>*>(add + col);
 #pragma unroll
-          for (int j = 0; j < V; ++j) z[i * V + j] = fmaf(rest[i * V + j], x.v[j], z[i * V + j]);
+          for (int j = 0; j < V; ++j)      // (a NaN logit that was not selected must not reach its column)
+            if (x.v[j] != 0.0f) z[i * V + j] = fmaf(rest[i * V + j], x.v[j], z[i * V + j]);
         }
       }
       Gr::sync();

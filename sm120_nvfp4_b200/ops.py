@@ -8,6 +8,7 @@ host to validate them (grouped_gemm_ops.cpp:113-135 forces a device synchronisat
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -668,24 +669,27 @@ def quantize_fp8(x: torch.Tensor, *, swiglu: bool = False, output: Optional[torc
         _check(False, "x must be a contiguous FP16, BF16 or FP32 CUDA matrix")
     rows, k = x.shape
     if swiglu:
-        _check(k % 2 == 0, "x must hold gate and up columns")
+        if not (k % 2 == 0):
+            _check(False, "x must hold gate and up columns")
         k //= 2
-    _check(k > 0 and k % 16 == 0, "K must be a positive multiple of 16")
+    if not (k > 0 and k % 16 == 0):
+        _check(False, "K must be a positive multiple of 16")
     source = x.data_ptr()
-    _check(source % 16 == 0, "x must be 16-byte aligned")
+    if not (source % 16 == 0):
+        _check(False, "x must be 16-byte aligned")
     index = x.get_device()
     if output is None:
         output = x.new_empty((rows, k), dtype=_FP8)
     else:
         _on_device(index, (output,), ("output",))
-        _check(output.dtype in _FP8_STORAGE and output.shape == (rows, k) and output.data_ptr() % 16 == 0,
-               "output must be 16-byte aligned float8_e4m3fn (or uint8) [rows, K]")
+        if not (output.dtype in _FP8_STORAGE and output.shape == (rows, k) and output.data_ptr() % 16 == 0):
+            _check(False, "output must be 16-byte aligned float8_e4m3fn (or uint8) [rows, K]")
     if output_scale is None:
         output_scale = x.new_empty((rows, _blocks_128(k)), dtype=torch.float32)
     else:
         _on_device(index, (output_scale,), ("output_scale",))
-        _check(output_scale.dtype == torch.float32 and output_scale.shape == (rows, _blocks_128(k)),
-               "output_scale must be float32 [rows, ceil(K/128)]")
+        if not (output_scale.dtype == torch.float32 and output_scale.shape == (rows, _blocks_128(k))):
+            _check(False, "output_scale must be float32 [rows, ceil(K/128)]")
     if rows:
         _launch(index, "b200_nvfp4_fp8_quantize_rows", output.data_ptr(), output_scale.data_ptr(), source, rows, k, kind,
                 int(swiglu))
@@ -697,14 +701,17 @@ def _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output, names):
     _on_device(index, (x, weight, x_scale, weight_scale), names)
     if x.dtype not in _FP8_STORAGE or weight.dtype not in _FP8_STORAGE:
         _check(False, f"{names[0]} and {names[1]} must be float8_e4m3fn (or raw uint8 codes)")
-    _check(x_scale.dtype == torch.float32 and weight_scale.dtype == torch.float32, "scales must be float32")
+    if not (x_scale.dtype == torch.float32 and weight_scale.dtype == torch.float32):
+        _check(False, "scales must be float32")
     shape = weight.shape
     n, k = shape[-2], shape[-1]
     if x.dim() != 2 or x.shape[1] != k:
         _check(False, f"{names[0]} and {names[1]} must share K")
     rows = x.shape[0]
-    _check(k > 0 and k % 16 == 0, "K must be a positive multiple of 16")
-    _check(n > 0 and n % 8 == 0, "N must be a positive multiple of 8")
+    if not (k > 0 and k % 16 == 0):
+        _check(False, "K must be a positive multiple of 16")
+    if not (n > 0 and n % 8 == 0):
+        _check(False, "N must be a positive multiple of 8")
     kb = _blocks_128(k)
     if x_scale.shape != (rows, kb):
         _check(False, f"{names[2]} must be [rows, ceil(K/128)]")
@@ -713,13 +720,15 @@ def _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output, names):
     if x.data_ptr() % 16 or weight.data_ptr() % 16:
         _check(False, f"{names[0]} and {names[1]} must be 16-byte aligned")
     if output is None:
-        _check(out_dtype in _FP8_OUT, "out_dtype must be float16, bfloat16 or float32")
+        if not (out_dtype in _FP8_OUT):
+            _check(False, "out_dtype must be float16, bfloat16 or float32")
         output = x.new_empty((rows, n), dtype=out_dtype)
     else:
         _on_device(index, (output,), ("output",))
-        _check(output.dtype in _FP8_OUT and output.shape == (rows, n) and output.data_ptr() % 16 == 0,
-               "output must be a 16-byte aligned FP16, BF16 or FP32 matrix [rows, N]")
-        _check(out_dtype is None or out_dtype == output.dtype, "out_dtype does not match output")
+        if not (output.dtype in _FP8_OUT and output.shape == (rows, n) and output.data_ptr() % 16 == 0):
+            _check(False, "output must be a 16-byte aligned FP16, BF16 or FP32 matrix [rows, N]")
+        if not (out_dtype is None or out_dtype == output.dtype):
+            _check(False, "out_dtype does not match output")
     return index, rows, n, k, output
 
 
@@ -734,8 +743,10 @@ def fp8_gemm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: t
     Not differentiable. The gradient with respect to the input is the same product: quantize_fp8(grad)
     times b.t().contiguous() with b_scale.t().contiguous().
     """
-    _check(a.is_cuda, "a must be a CUDA tensor")
-    _check(b.dim() == 2, "b must be [N, K]")
+    if not (a.is_cuda):
+        _check(False, "a must be a CUDA tensor")
+    if not (b.dim() == 2):
+        _check(False, "b must be [N, K]")
     if out_dtype is None and output is None:
         out_dtype = torch.float16
     index, m, n, k, out = _fp8_operands(a, b, a_scale, b_scale, out_dtype, output, ("a", "b", "a_scale", "b_scale"))
@@ -754,18 +765,22 @@ def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tenso
     the device; the ranges must not overlap. Rows that belong to no group keep what `output` held (without
     `output` they are undefined). groups <= 256; otherwise as fp8_gemm.
     """
-    _check(x.is_cuda, "x must be a CUDA tensor")
-    _check(weight.dim() == 3, "weight must be [groups, N, K]")
+    if not (x.is_cuda):
+        _check(False, "x must be a CUDA tensor")
+    if not (weight.dim() == 3):
+        _check(False, "weight must be [groups, N, K]")
     if out_dtype is None and output is None:
         out_dtype = torch.float16
     index, rows, n, k, out = _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output,
                                            ("x", "weight", "x_scale", "weight_scale"))
     groups = weight.shape[0]
-    _check(0 < groups <= 256, "number of groups must be in [1, 256]")
+    if not (0 < groups <= 256):
+        _check(False, "number of groups must be in [1, 256]")
     _on_device(index, (seqlens, cu_seqlens), ("seqlens", "cu_seqlens"))
-    _check(seqlens.dtype == torch.int32 and cu_seqlens.dtype == torch.int32, "seqlens and cu_seqlens must be int32")
-    _check(seqlens.numel() == groups and cu_seqlens.numel() == groups + 1,
-           "seqlens / cu_seqlens lengths are inconsistent with the number of groups")
+    if not (seqlens.dtype == torch.int32 and cu_seqlens.dtype == torch.int32):
+        _check(False, "seqlens and cu_seqlens must be int32")
+    if not (seqlens.numel() == groups and cu_seqlens.numel() == groups + 1):
+        _check(False, "seqlens / cu_seqlens lengths are inconsistent with the number of groups")
     if rows:
         _launch(index, "b200_nvfp4_fp8_grouped_gemm", out.data_ptr(), x.data_ptr(), weight.data_ptr(), seqlens.data_ptr(),
                 cu_seqlens.data_ptr(), x_scale.data_ptr(), weight_scale.data_ptr(), groups, rows, n, k, 0,
@@ -786,18 +801,25 @@ def _check_router(logits, topk_ids, cu_seqlens, scoring):
     t, e = logits.shape
     index = logits.get_device()
     _on_device(index, (topk_ids,), ("topk_ids",))
-    _check(topk_ids.dtype == torch.int32 and topk_ids.dim() == 2 and topk_ids.shape[0] == t,
-           "topk_ids must be int32 [num_tokens, num_topk]")
+    if not (topk_ids.dtype == torch.int32 and topk_ids.dim() == 2 and topk_ids.shape[0] == t):
+        _check(False, "topk_ids must be int32 [num_tokens, num_topk]")
     k = topk_ids.shape[1]
-    _check(0 < k <= e <= 4096, "need 0 < num_topk <= num_experts <= 4096")
-    _check(scoring in _SCORING, "scoring must be 'sigmoid' or 'softmax'")
+    if not (0 < k <= e <= 4096):
+        _check(False, "need 0 < num_topk <= num_experts <= 4096")
+    if not (scoring in _SCORING):
+        _check(False, "scoring must be 'sigmoid' or 'softmax'")
     sequences = 1
     if cu_seqlens is not None:
         _on_device(index, (cu_seqlens,), ("cu_seqlens",))
-        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 2 <= cu_seqlens.numel() <= 65537,
-               "cu_seqlens must be int32 [num_sequences + 1] with at most 65536 sequences")
+        if not (cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and 2 <= cu_seqlens.numel() <= 65537):
+            _check(False, "cu_seqlens must be int32 [num_sequences + 1] with at most 65536 sequences")
         sequences = cu_seqlens.numel() - 1
     return index, kind, t, e, k, sequences
+
+
+@functools.lru_cache(maxsize=1024)
+def _balance_workspace(t: int, e: int, sequences: int) -> int:
+    return _lib.lib().b200_nvfp4_moe_balance_loss_workspace_bytes(t, e, sequences)
 
 
 def _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha):
@@ -805,7 +827,7 @@ def _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha):
     loss = logits.new_empty((), dtype=torch.float32)
     counts = topk_ids.new_empty((sequences, e))
     slope = logits.new_empty((sequences, e), dtype=torch.float32)
-    need = _lib.lib().b200_nvfp4_moe_balance_loss_workspace_bytes(t, e, sequences)
+    need = _balance_workspace(t, e, sequences)
     workspace = logits.new_empty(need, dtype=torch.uint8)
     _launch(index, "b200_nvfp4_moe_balance_loss", loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), logits.data_ptr(),
             topk_ids.data_ptr(), _ptr(cu_seqlens), t, e, k, sequences, kind, _SCORING[scoring], float(alpha),
@@ -826,20 +848,24 @@ def router_backward(logits: torch.Tensor, topk_ids: torch.Tensor, *, topk_weight
     [0, E) are empty; slots of a token that name the same expert add up.
     """
     index, kind, t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
-    _check(grad_weights is not None or slope is not None, "grad_weights or slope must be given")
+    if not (grad_weights is not None or slope is not None):
+        _check(False, "grad_weights or slope must be given")
     if grad_weights is not None:
-        _check(topk_weights is not None, "grad_weights needs topk_weights")
+        if not (topk_weights is not None):
+            _check(False, "grad_weights needs topk_weights")
         _on_device(index, (topk_weights, grad_weights), ("topk_weights", "grad_weights"))
-        _check(topk_weights.dtype == torch.float32 and grad_weights.dtype == torch.float32 and
-               topk_weights.shape == topk_ids.shape and grad_weights.shape == topk_ids.shape,
-               "topk_weights and grad_weights must be float32 [T, k]")
+        if not (topk_weights.dtype == torch.float32 and grad_weights.dtype == torch.float32 and
+                topk_weights.shape == topk_ids.shape and grad_weights.shape == topk_ids.shape):
+            _check(False, "topk_weights and grad_weights must be float32 [T, k]")
     if slope is not None:
-        _check(grad_loss is not None, "slope needs grad_loss")
+        if not (grad_loss is not None):
+            _check(False, "slope needs grad_loss")
         _on_device(index, (slope,), ("slope",))
-        _check(slope.dtype == torch.float32 and slope.shape == (sequences, e),
-               "slope must be float32 [num_sequences, num_experts]")
-        _check(grad_loss.is_cuda and grad_loss.get_device() == index and grad_loss.dtype == torch.float32 and
-               grad_loss.numel() == 1, "grad_loss must be one float32 on the device of the logits")
+        if not (slope.dtype == torch.float32 and slope.shape == (sequences, e)):
+            _check(False, "slope must be float32 [num_sequences, num_experts]")
+        if not (grad_loss.is_cuda and grad_loss.get_device() == index and grad_loss.dtype == torch.float32 and
+                grad_loss.numel() == 1):
+            _check(False, "grad_loss must be one float32 on the device of the logits")
     grad = torch.empty_like(logits)
     if t:
         _launch(index, "b200_nvfp4_moe_router_backward", grad.data_ptr(), logits.data_ptr(), topk_ids.data_ptr(),

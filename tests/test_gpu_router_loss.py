@@ -318,3 +318,54 @@ def test_captured_and_on_another_stream(ops):
     eager = step()
     for _, held in graphs:
         assert all(torch.equal(a, b) for a, b in zip(eager, held))
+
+
+def test_nan_in_masked_and_unselected_places(ops):
+    """NaN and infinite logits of masked tokens, of tokens behind the last sequence and (through the
+    weights alone) of experts that were not selected change nothing."""
+    t, e, k = 40, 24, 3
+    z, ids, _, gw = case(t, e, k, 0, 11, masked=0.0)
+    cu = torch.tensor([2, 20, 30], dtype=torch.int32)
+    ids[5] = -1
+    w = weights_of(z, ids).nan_to_num()
+    clean = z.clone()
+    z[5], z[0], z[35] = float("nan"), float("inf"), float("nan")
+    gw[5] = float("nan")                                           # its slots are empty
+    one = torch.ones((), device="cuda")
+    loss, counts, slope = ops.router_balance_loss(z.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
+    want = ops.router_balance_loss(clean.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
+    assert all(torch.equal(a, b) for a, b in zip((loss, counts, slope), want)) and torch.isfinite(loss)
+    grad = ops.router_backward(z.cuda(), ids.cuda(), slope=slope, grad_loss=one, cu_seqlens=cu.cuda())
+    assert torch.equal(grad, ops.router_backward(clean.cuda(), ids.cuda(), slope=slope, grad_loss=one, cu_seqlens=cu.cuda()))
+    assert (grad[[0, 1, 5, 30, 35, 39]] == 0).all()
+    both = ops.router_backward(z.cuda(), ids.cuda(), topk_weights=w.cuda(), grad_weights=gw.cuda(), slope=slope, grad_loss=one,
+                               cu_seqlens=cu.cuda())
+    assert (both[5] == 0).all()
+    row = clean.clone()
+    unselected = [x for x in range(e) if x not in ids[7].tolist()]
+    row[7, unselected[0]] = float("nan")
+    got = ops.router_backward(row.cuda(), ids.cuda(), topk_weights=w.cuda(), grad_weights=gw.cuda())
+    assert torch.equal(got, ops.router_backward(clean.cuda(), ids.cuda(), topk_weights=w.cuda(), grad_weights=gw.cuda()))
+    assert (got[7, unselected] == 0).all()
+
+
+def test_autograd_captured_into_a_graph(ops):
+    t, e, k = 200, 64, 4
+    z, _, cu, gw = case(t, e, k, 3, 12)
+    leaf, cu, gw = z.cuda().requires_grad_(), cu.cuda(), gw.cuda()
+
+    def step():
+        _, weights, loss, _ = ops.router_topk_balanced(leaf, k, cu_seqlens=cu)
+        return torch.autograd.grad((weights * gw).sum() + loss, leaf)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, eager)
