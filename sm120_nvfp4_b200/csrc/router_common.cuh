@@ -27,7 +27,7 @@ __device__ __forceinline__ void from_float(float x, float* p) { *p = x; }
 __device__ __forceinline__ void from_float(float x, __half* p) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void from_float(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
 
-// 1 / x to one ulp (0 for infinite x; x is at least 1 here).
+// 1 / x to one ulp (0 for infinite x, infinity for 0).
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -110,24 +110,20 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
 }
 
-template <typename T, int V, int NV, int G>
+template <typename T, int V, int NV, int G, bool kLoose = V == 1 && sizeof(T) == 2>
 struct RowQueue {
   using Part = Vec<T, V>;
   static constexpr size_t kBytes = static_cast<size_t>(kDepth) * NV * kThreads * sizeof(Part);   // per block
   static constexpr int kStage = NV * kThreads * static_cast<int>(sizeof(Part));
   uint8_t* mine;                                            // this thread's first part
-  __device__ __forceinline__ explicit RowQueue(void* smem) : mine(static_cast<uint8_t*>(smem) + threadIdx.x * sizeof(Part)) {}
+  __device__ __forceinline__ RowQueue(void* smem, const T*, int, int) : mine(static_cast<uint8_t*>(smem) + threadIdx.x * sizeof(Part)) {}
   __device__ __forceinline__ void push(int stage, const T* row, int experts, int lane) {
     uint8_t* to = mine + stage * kStage;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * G + lane) * V;
-      if (col < experts) {
-        if constexpr (sizeof(Part) >= 4)
-          copy_async<static_cast<int>(sizeof(Part))>(static_cast<uint32_t>(__cvta_generic_to_shared(to + i * kThreads * sizeof(Part))), row + col);
-        else
-          *reinterpret_cast<Part*>(to + i * kThreads * sizeof(Part)) = *reinterpret_cast<const Part*>(row + col);
-      }
+      if (col < experts)
+        copy_async<static_cast<int>(sizeof(Part))>(static_cast<uint32_t>(__cvta_generic_to_shared(to + i * kThreads * sizeof(Part))), row + col);
     }
   }
   // Columns past the end are -infinity, whose score is zero; no copy ever touches them.
@@ -141,7 +137,8 @@ struct RowQueue {
       for (int stage = 0; stage < kDepth; ++stage) *reinterpret_cast<Part*>(mine + stage * kStage + i * kThreads * sizeof(Part)) = rest;
     }
   }
-  __device__ __forceinline__ void pop(int stage, float (&z)[V * NV]) const {
+  // the row of the step whose copies queue_wait() has waited for
+  __device__ __forceinline__ void pop(int stage, const T*, float (&z)[V * NV], int, int) const {
     const uint8_t* from = mine + stage * kStage;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -149,6 +146,48 @@ struct RowQueue {
 #pragma unroll
       for (int j = 0; j < V; ++j) z[i * V + j] = to_float(w.v[j]);
     }
+  }
+};
+
+// 16-bit rows that cannot be copied by the column (asynchronous copies have 4 bytes at least): the group
+// copies the 16-byte chunks that a row lies in, clipped to the matrix, and its threads pick their columns
+// i * G + lane out of them. (FP32 rows do better with copies of 4 bytes: 65536 x 255 33 against 37 us.)
+template <typename T, int NV, int G>
+struct RowQueue<T, 1, NV, G, true> {
+  static constexpr int kRow = (NV * G * static_cast<int>(sizeof(T)) + 15) / 16 * 16 + 16;
+  static constexpr size_t kBytes = static_cast<size_t>(kDepth) * Group<G>::kPerBlock * kRow;
+  uint8_t* mine;                                            // this group's first row
+  const uint8_t *first, *last;                              // ends of the matrix
+  __device__ __forceinline__ RowQueue(void* smem, const T* matrix, int tokens, int experts)
+      : mine(static_cast<uint8_t*>(smem) + Group<G>::index() * kDepth * kRow),
+        first(reinterpret_cast<const uint8_t*>(matrix)),
+        last(reinterpret_cast<const uint8_t*>(matrix + static_cast<long long>(tokens) * experts)) {}
+  __device__ __forceinline__ void push(int stage, const T* row, int experts, int lane) {
+    const uint8_t* begin = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(row) & ~static_cast<uintptr_t>(15));
+    const uint8_t* end = reinterpret_cast<const uint8_t*>(row + experts);
+    for (int c = lane * 16; begin + c < end; c += G * 16) {
+      uint8_t* to = mine + stage * kRow + c;
+      if (begin + c >= first) {
+        const int bytes = static_cast<int>(min(static_cast<long long>(16), static_cast<long long>(last - (begin + c))));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                     "l"(begin + c), "r"(bytes)
+                     : "memory");
+      } else {                                              // the chunk that starts before an unaligned matrix
+        for (const uint8_t* x = first; x < begin + c + 16 && x < end; x += sizeof(T))
+          *reinterpret_cast<T*>(to + (x - (begin + c))) = *reinterpret_cast<const T*>(x);
+      }
+    }
+  }
+  __device__ __forceinline__ void fill_rest(int, int) {}
+  __device__ __forceinline__ void pop(int stage, const T* row, float (&z)[NV], int experts, int lane) const {
+    Group<G>::sync();                                       // the other threads' copies have landed too
+    const T* from = reinterpret_cast<const T*>(mine + stage * kRow + (reinterpret_cast<uintptr_t>(row) & 15));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = i * G + lane;
+      z[i] = col < experts ? to_float(from[col]) : __int_as_float(0xff800000);
+    }
+    Group<G>::sync();                                       // before the place is filled again
   }
 };
 
@@ -203,6 +242,8 @@ int dispatch_width(int experts, bool quads, Args... args) {
     return Launch<T, 4, 4, 256>::run(args...);
   }
   if (experts <= 64) return Launch<T, 1, 8, 8>::run(args...);
+  if (experts <= 128) return Launch<T, 1, 16, 8>::run(args...);
+  if (experts <= 192) return Launch<T, 1, 12, 16>::run(args...);
   if (experts <= 256) return Launch<T, 1, 16, 16>::run(args...);
   if (experts <= 512) return Launch<T, 1, 16, 32>::run(args...);
   return Launch<T, 1, 16, 256>::run(args...);

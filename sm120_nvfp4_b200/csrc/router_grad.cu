@@ -43,7 +43,7 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
   __shared__ float scratch[kWarps];
   const int lane = Gr::lane();
   using Rows = RowQueue<T, V, NV, G>;
-  Rows rows(s_raw);
+  Rows rows(s_raw, logits, p.tokens, p.experts);
   rows.fill_rest(p.experts, lane);
   WordQueue<int> first_ids(s_raw + Rows::kBytes);
   WordQueue<float> first_w(s_raw + Rows::kBytes + WordQueue<int>::kBytes);
@@ -91,10 +91,11 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
   long long slots = static_cast<long long>(t) * p.topk, slots_ahead = slots;
   T* out = grad + static_cast<long long>(t) * p.experts;
   const T* row = logits + static_cast<long long>(t) * p.experts;
+  const T* row_ahead = row;
   int ahead = t;                                           // the next token to be fetched
   auto fetch = [&](int stage) {
     if (ahead < end) {
-      rows.push(stage, row, p.experts, lane);
+      rows.push(stage, row_ahead, p.experts, lane);
       if (lane < p.topk) {
         first_ids.push(stage, p.ids + slots_ahead + lane);
         if (through_weights) {
@@ -105,7 +106,7 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
     }
     queue_commit();
     ahead += Gr::kPerWarp;
-    row += row_step;
+    row_ahead += row_step;
     slots_ahead += slot_step;
   };
   for (int i = 0; i < kDepth - 1; ++i) fetch(i);
@@ -119,7 +120,7 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
     queue_wait();
     const bool in = t < end;
     float z[N];
-    rows.pop(stage, z);
+    rows.pop(stage, row, z, p.experts, lane);
     int id = -1;
     float w = 0.0f, gw = 0.0f;
     if (in && lane < p.topk) {
@@ -150,24 +151,26 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
     const bool inside = Gr::any(mine) && in && through_loss && t >= s_begin && t < s_end;
     t += Gr::kPerWarp;
 
-    // s = 1 / (1 + u), 1 - s = u s with u = e^-z, held below 2^126 so that neither overflows
-    float sc[N], rest[N];
+    // s = 1 / (1 + u), 1 - s = u s with u = e^-z, held below 2^126 so that neither overflows. What is kept
+    // is s (1 - s) in `both`, which the gradient of the loss has as a factor, and 1 - s.
+    float both[N], rest[N];
     float sum = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float u = __expf(min_nan(-z[i], 87.0f));
       const float x = reciprocal(1.0f + u);
       rest[i] = u * x;
-      sc[i] = z[i] <= -87.0f ? 0.0f : x;
-      sum += sc[i];
-      dot = fmaf(d[i], sc[i], dot);
+      const float sc = z[i] <= -87.0f ? 0.0f : x;
+      both[i] = sc * rest[i];
+      sum += sc;
+      dot = fmaf(d[i], sc, dot);
     }
     if (through_loss) {
       sum = Gr::sum(sum, scratch);
       dot = Gr::sum(dot, scratch);
       const bool by_max = inside && (p.softmax || !(sum >= kMinSum));
-      float inv = __fdividef(1.0f, sum);
-      if (Gr::any_here(by_max)) {      // softmax, or scores that all vanish (they are e^z, and 1 - s is 1)
+      float inv = reciprocal(sum);
+      if (Gr::any_here(by_max)) {      // softmax, or scores that all vanish: they are e^z then
         const float other = exponentials<N, G>(z, scratch);
         float dot2 = 0.0f;
 #pragma unroll
@@ -176,16 +179,12 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         inv = by_max ? other : inv;
         dot = by_max ? dot2 : dot;
 #pragma unroll
-        for (int i = 0; i < N; ++i) sc[i] = by_max ? z[i] : sc[i];
+        for (int i = 0; i < N; ++i) both[i] = by_max ? (p.softmax ? z[i] : z[i] * rest[i]) : both[i];
       }
-      dot *= inv;
-      const float by = g * inv;
+      // g p (1 - s) (slope - dot) with the row's constants multiplied out
+      const float by = g * inv, minus = -by * (dot * inv);
 #pragma unroll
-      for (int i = 0; i < N; ++i) z[i] = by * sc[i] * (d[i] - dot);
-      if (!p.softmax) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) z[i] *= rest[i];
-      }
+      for (int i = 0; i < N; ++i) z[i] = both[i] * fmaf(by, d[i], minus);
       if (Gr::any_here(!inside)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) z[i] = inside ? z[i] : 0.0f;
@@ -254,6 +253,7 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         }
       }
     }
+    row += row_step;
     out += row_step;
     slots += slot_step;
   }

@@ -72,7 +72,7 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
   const int lane = Gr::lane();
   float* s_dyn = reinterpret_cast<float*>(s_raw);
   using Rows = RowQueue<T, V, NV, G>;
-  Rows rows(s_raw);
+  Rows rows(s_raw, logits, p.tokens, p.experts);
   rows.fill_rest(p.experts, lane);
   WordQueue<int> first_ids(s_raw + Rows::kBytes);
   int* s_counts = reinterpret_cast<int*>(s_raw + p.counts_at);
@@ -100,18 +100,19 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
   int t = lo + Gr::index();                                // the next token to be worked on
   int ahead = t;                                           // ... to be fetched
   const T* row = logits + static_cast<long long>(t) * p.experts;
+  const T* row_ahead = row;
   const int* slots = p.ids + static_cast<long long>(t) * p.topk;
   const long long row_step = static_cast<long long>(Gr::kPerBlock) * p.experts;
   const int slot_step = Gr::kPerBlock * p.topk;
   const int* slots_ahead = slots;
   auto fetch = [&](int stage) {
     if (ahead < hi) {
-      rows.push(stage, row, p.experts, lane);
+      rows.push(stage, row_ahead, p.experts, lane);
       if (lane < p.topk) first_ids.push(stage, slots_ahead + lane);
     }
     queue_commit();
     ahead += Gr::kPerBlock;
-    row += row_step;
+    row_ahead += row_step;
     slots_ahead += slot_step;
   };
   auto count = [&](int id) {
@@ -127,12 +128,13 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
     fetch((step + kDepth - 1) & (kDepth - 1));
     queue_wait();
     float z[N];
-    rows.pop(stage, z);
+    rows.pop(stage, row, z, p.experts, lane);
     const bool in = t < hi;
     bool mine = in && lane < p.topk && count(first_ids.pop(stage));
     if (in)
       for (int j = lane + G; j < p.topk; j += G) mine |= count(slots[j]);
     t += Gr::kPerBlock;
+    row += row_step;
     slots += slot_step;
     const bool live = Gr::any(mine);
     if (!Gr::any_here(live)) continue;

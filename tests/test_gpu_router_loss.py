@@ -369,3 +369,22 @@ def test_autograd_captured_into_a_graph(ops):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,k", [(70, 179, 5), (33, 255, 8), (9, 101, 7), (600, 63, 2), (19, 387, 4), (11, 777, 3)])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_rows_of_any_alignment(ops, t, e, k, offset, dtype):
+    """Odd numbers of experts, and matrices that start off a 16-byte boundary with NaN on both sides."""
+    z, ids, cu, gw = case(t, e, k, 2, t + e + offset, dtype)
+    store = torch.full((t * e + 32,), float("nan"), dtype=dtype)
+    store[offset:offset + t * e] = z.flatten()
+    off = store.cuda()[offset:offset + t * e].view(t, e)
+    w = weights_of(z, ids)
+    loss, counts, slope = ops.router_balance_loss(off, ids.cuda(), cu_seqlens=cu.cuda())
+    wl, wc, ws, live, seq = reference(z, ids, cu, "sigmoid", 1.0)
+    assert torch.equal(counts.cpu().long(), wc) and abs(float(loss) - float(wl)) <= float(wl) * 2.0 ** -15
+    got = ops.router_backward(off, ids.cuda(), topk_weights=w.cuda(), grad_weights=gw.cuda(), slope=slope,
+                              grad_loss=torch.ones((), device="cuda"), cu_seqlens=cu.cuda())
+    want, size = reference_grad(z, ids, w, gw, cu, ws, 1.0, "sigmoid", live, seq)
+    compare_grad(got, want, size, z)
