@@ -6,11 +6,13 @@ ops raises. The library is built in-tree by sm120_nvfp4_b200.build.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
 _LIB_PATH = _PKG / "libb200_nvfp4.so"
 _lib = None
+_calls = None
 
 STATUS_SUCCESS = 0
 STATUS_INVALID_ARGUMENT = 1
@@ -100,6 +102,18 @@ def lib():
             fn.argtypes = argtypes
         _lib = L
     return _lib
+
+
+def calls():
+    """The extension module that calls some entry points without ctypes (csrc/torch_calls.cpp)."""
+    global _calls
+    if _calls is None:
+        lib()
+        from . import build as _build
+        if not _build.CALLS.exists():
+            _build.build_calls()
+        _calls = importlib.import_module("._calls", __package__)
+    return _calls
 
 
 def status_string(status: int) -> str:

@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -23,6 +24,9 @@ SOURCES = ["gemm.cu", "gemm_splitk_static.cu", "gemm_host.cu", "fp8_gemm.cu", "f
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=hidden", "-Xptxas", "-v",
               f"-I{ROOT / 'include'}", f"-I{CSRC}"]
+
+
+CALLS = PKG / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def _nvcc() -> str:
@@ -74,5 +78,28 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return OUT
 
 
+def build_calls(force: bool = False) -> Path:
+    """The extension module of csrc/torch_calls.cpp: host code only, against the installed torch and this
+    package's library (found beside it at run time)."""
+    src = CSRC / "torch_calls.cpp"
+    if not (force or _stale(CALLS, [src, ROOT / "include" / "b200_nvfp4.h"])):
+        return CALLS
+    import torch
+    from torch.utils import cpp_extension
+    lib = build()
+    includes = [*cpp_extension.include_paths(), os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include"),
+                sysconfig.get_path("include"), str(ROOT / "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes), str(src),
+           "-o", str(CALLS), f"-L{libs}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+           f"-L{lib.parent}", f"-l:{lib.name}", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    return CALLS
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_calls(force="--force" in sys.argv))

@@ -8,7 +8,6 @@ host to validate them (grouped_gemm_ops.cpp:113-135 forces a device synchronisat
 """
 from __future__ import annotations
 
-import functools
 from typing import Optional, Tuple
 
 import torch
@@ -621,21 +620,14 @@ _FP8_OUT = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 _INPUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-# The checks below run on every call, and a small call is all checks and launch: they read integers, build no
-# messages unless one is needed, and take the stream and device by their raw numbers.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
+# A small call is all checks, allocations and launch. The usual call therefore goes through an extension
+# module (_lib.calls(): the same checks, outputs and entry points in C++), which declines anything else by
+# returning None; what it declines comes the long way below, which says what is wrong.
 
 def _launch(index: int, function: str, *args) -> None:
-    """Calls a C-ABI function with torch's current stream of device `index` as its last argument; the device
-    is switched only where it is not the current one."""
-    call = getattr(_lib.lib(), function)
-    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
-    if torch.cuda.current_device() == index:
-        status = call(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            status = call(*args, stream)
+    """Calls a C-ABI function on device `index`, with torch's current stream there as its last argument."""
+    with torch.cuda.device(index):
+        status = getattr(_lib.lib(), function)(*args, torch.cuda.current_stream(index).cuda_stream)
     if status:
         raise RuntimeError(f"{function} failed: {_lib.status_string(status)}")
 
@@ -664,6 +656,9 @@ def quantize_fp8(x: torch.Tensor, *, swiglu: bool = False, output: Optional[torc
     step between the two products of an expert. A block with a NaN or an infinity gets a NaN or
     infinite scale. Not differentiable.
     """
+    done = _lib.calls().quantize_fp8(x, swiglu, output, output_scale)
+    if done is not None:
+        return done
     kind = _INPUT.get(x.dtype)
     if not (kind is not None and x.is_cuda and x.dim() == 2 and x.is_contiguous()):
         _check(False, "x must be a contiguous FP16, BF16 or FP32 CUDA matrix")
@@ -743,6 +738,9 @@ def fp8_gemm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: t
     Not differentiable. The gradient with respect to the input is the same product: quantize_fp8(grad)
     times b.t().contiguous() with b_scale.t().contiguous().
     """
+    done = _lib.calls().fp8_gemm(a, b, a_scale, b_scale, out_dtype, output)
+    if done is not None:
+        return done
     if not (a.is_cuda):
         _check(False, "a must be a CUDA tensor")
     if not (b.dim() == 2):
@@ -765,6 +763,9 @@ def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tenso
     the device; the ranges must not overlap. Rows that belong to no group keep what `output` held (without
     `output` they are undefined). groups <= 256; otherwise as fp8_gemm.
     """
+    done = _lib.calls().fp8_grouped_gemm(x, weight, seqlens, cu_seqlens, x_scale, weight_scale, out_dtype, output)
+    if done is not None:
+        return done
     if not (x.is_cuda):
         _check(False, "x must be a CUDA tensor")
     if not (weight.dim() == 3):
@@ -817,17 +818,16 @@ def _check_router(logits, topk_ids, cu_seqlens, scoring):
     return index, kind, t, e, k, sequences
 
 
-@functools.lru_cache(maxsize=1024)
-def _balance_workspace(t: int, e: int, sequences: int) -> int:
-    return _lib.lib().b200_nvfp4_moe_balance_loss_workspace_bytes(t, e, sequences)
-
-
 def _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha):
+    if scoring in _SCORING:
+        done = _lib.calls().balance_loss(logits, topk_ids, cu_seqlens, _SCORING[scoring], alpha)
+        if done is not None:
+            return done
     index, kind, t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
     loss = logits.new_empty((), dtype=torch.float32)
     counts = topk_ids.new_empty((sequences, e))
     slope = logits.new_empty((sequences, e), dtype=torch.float32)
-    need = _balance_workspace(t, e, sequences)
+    need = _lib.lib().b200_nvfp4_moe_balance_loss_workspace_bytes(t, e, sequences)
     workspace = logits.new_empty(need, dtype=torch.uint8)
     _launch(index, "b200_nvfp4_moe_balance_loss", loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), logits.data_ptr(),
             topk_ids.data_ptr(), _ptr(cu_seqlens), t, e, k, sequences, kind, _SCORING[scoring], float(alpha),
@@ -847,6 +847,11 @@ def router_backward(logits: torch.Tensor, topk_ids: torch.Tensor, *, topk_weight
     `scoring` is that of the loss; the weights are router_topk's (sigmoid). Slots with an id outside
     [0, E) are empty; slots of a token that name the same expert add up.
     """
+    if scoring in _SCORING:
+        done = _lib.calls().router_backward(logits, topk_ids, topk_weights, grad_weights, slope, grad_loss, cu_seqlens,
+                                            _SCORING[scoring])
+        if done is not None:
+            return done
     index, kind, t, e, k, sequences = _check_router(logits, topk_ids, cu_seqlens, scoring)
     if not (grad_weights is not None or slope is not None):
         _check(False, "grad_weights or slope must be given")

@@ -412,3 +412,37 @@ def test_a_wait_that_runs_out_is_reported(ops, L, tile, splits, m):
     assert torch.equal(ops.fp8_gemm(a, b, sa, sb), want)
     code = ctypes.c_int(-1)
     assert L.b200_nvfp4_device_error(ctypes.byref(code)) == 0 and code.value == 0
+
+
+class _Declines:
+    """Stands in for the extension module and declines every call."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_the_long_way_gives_the_same_results(ops, monkeypatch):
+    """What the extension module declines goes through ctypes: same outputs, same `output` tensors."""
+    from sm120_nvfp4_b200 import _lib
+    a, sa = codes(20, 400, 1)
+    b, sb = weight(136, 400, 2)
+    w, sw = b.view(torch.uint8).view(1, 136, 400).view(E4M3), sb.view(1, *sb.shape)
+    n = torch.tensor([15], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 15], dtype=torch.int32, device="cuda")
+    x = torch.randn((20, 800), device="cuda", dtype=torch.float16)
+    z = torch.randn((20, 16), device="cuda")
+    ids, weights = ops.router_topk(z, 2)
+
+    def everything():
+        held = torch.full((20, 136), 3.0, dtype=torch.float32, device="cuda")
+        loss, counts, slope = ops.router_balance_loss(z, ids, alpha=0.5)
+        return [ops.fp8_gemm(a, b, sa, sb), ops.fp8_gemm(a, b, sa, sb, out_dtype=torch.bfloat16),
+                ops.fp8_gemm(a, b, sa, sb, output=torch.empty((20, 136), device="cuda")),
+                ops.fp8_grouped_gemm(a, w, n, cu, sa, sw, output=held), *ops.quantize_fp8(x), *ops.quantize_fp8(x, swiglu=True),
+                *ops.quantize_fp8(x, output=torch.empty((20, 800), dtype=torch.uint8, device="cuda")),
+                loss, counts, slope, ops.router_backward(z, ids, topk_weights=weights, grad_weights=weights, slope=slope, grad_loss=loss)]
+
+    short = everything()
+    monkeypatch.setattr(_lib, "calls", lambda: _Declines())
+    for p, q in zip(short, everything()):
+        assert p.dtype == q.dtype and p.shape == q.shape and torch.equal(p.contiguous().view(-1).view(torch.uint8), q.contiguous().view(-1).view(torch.uint8))
