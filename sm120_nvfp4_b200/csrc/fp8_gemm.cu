@@ -138,12 +138,12 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
 
 // CTAs per tile over K: as many as still fit the GPU at once and leave each enough blocks of K to pay for the
 // exchange of partial tiles, which grows with the tile (us, tile / splits; 24 x 1024 x 1024: 16/1 6.3,
-// 16/4 5.9; 64 x 7168 x 2048: 64/1 10.6, 64/2 10.3; 128 x 7168 x 2048: 128/1 12.8, 128/2 14.8;
+// 16/4 5.9; 96 x 1024 x 1024: 64/1 7.6, 64/2 8.7; 64 x 7168 x 2048: 64/1 10.6, 64/2 10.3; 128 x 7168 x 2048: 128/1 12.8, 128/2 14.8;
 // 128 x 4096 x 7168: 128/1 29.5, 128/4 17.2).
 int pick_fp8_splits(const Fp8Problem& q, const DeviceInfo& dev, int tile) {
   const long long tasks = row_tiles(q, tile) * ((q.n + 127) / 128);
   const int kb = (q.k + kFp8BlockK - 1) / kFp8BlockK;
-  const int least = tile == 16 ? 2 : (tile == 128 ? 12 : 4);
+  const int least = tile == 16 ? 2 : (tile == 128 ? 12 : 8);
   for (int s = 8; s >= 2; s /= 2)
     if (tasks * s <= dev.sm_count && kb >= least * s) return s;
   return 1;

@@ -253,7 +253,14 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   const int task_step = splits > 1 ? total_tasks : static_cast<int>(gridDim.x);
   const int b_begin = kb * rank / splits, b_end = kb * (rank + 1) / splits;
   const uint32_t stage_u32 = ptx::smem_u32(smem);
-  bool met = false;             // this warp has waited for the cluster's set-up
+  // Threads of a cluster wait for each other twice: `met`, this warp has waited for the set-up of the others'
+  // barriers; `done`, it has said that it needs nothing of the others any more.
+  bool met = false, done = false;
+  // (a single row of tiles needs none of the divisions: they stood 0.6 us before the first load)
+  auto decode = [&](int task) {
+    if (one_group && total_mt == 1) return TileCoord{0, 0, task, 0};
+    return decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
+  };
 
   if (warp == kLoadWide || warp == kLoadNarrow) {
     const bool wide = warp == kLoadWide, rows_of_a = wide == kWide;
@@ -263,7 +270,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     uint32_t phase = 0;
     bool ok = true, withhold = wide && p.withhold_first_arrival != 0 && blockIdx.x == 0;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
-      const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
+      const TileCoord t = decode(task);
       const int row = rows_of_a ? s_row0[t.g] + t.mt * Cfg::kTileM : t.g * p.n + t.nt * Cfg::kTileN;
       for (int b = b_begin; b < b_end; ++b) {
         if (!ptx::mbar_wait(empty_u32 + 8 * stage, phase ^ 1, abort_flag, kWaitEmpty, p.wait_limit)) { ok = false; break; }
@@ -317,7 +324,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     // (A loader warp with asynchronous copies had the first panel ready 2000 cycles after the operands.)
     float next_scale[Cfg::kScales], next_w_scale = 0.0f;
     auto fetch_scales = [&](int task, int b0) {
-      const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
+      const TileCoord t = decode(task);
       const int left = s_rows[t.g] - t.mt * Cfg::kTileM;
       const int j = tid & 7;
       const float* src = p.a_scale + static_cast<long long>(s_row0[t.g] + t.mt * Cfg::kTileM) * kb + b0 + j;
@@ -334,7 +341,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     bool ok = true;
     if (first_task < total_tasks && b_begin < b_end) fetch_scales(first_task, b_begin);
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
-      const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
+      const TileCoord t = decode(task);
       // rows of A and output columns of the tile that exist; `valid` are those the registers run over
       const int rows_in = min(Cfg::kTileM, s_rows[t.g] - t.mt * Cfg::kTileM), cols_in = min(Cfg::kTileN, p.n - t.nt * Cfg::kTileN);
       const int valid = kWide ? cols_in : rows_in;
@@ -476,8 +483,10 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                                   ptx::map_to_cta(red_full_u32, d));
           }
         }
+        if (mine > 0 && !ptx::mbar_wait_cluster(red_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
+        ptx::cluster_arrive_relaxed();       // the others' copies have landed here (the wait is in the teardown)
+        done = true;
         if (mine > 0) {
-          if (!ptx::mbar_wait_cluster(red_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
           // partial sums in split order, two columns per thread
           auto reduce = [&](auto count) {
             constexpr int kSplits = decltype(count)::value;
@@ -541,11 +550,14 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     __syncwarp();
   }
 
-  // ---- teardown (a CTA of a cluster must outlive its copies: their receivers arrive after having got them)
-  if (splits > 1 && !met) ptx::cluster_wait();     // every thread waits once for the arrival at set-up
+  // ---- teardown. A CTA of a cluster must outlive its copies: their receivers arrive after having got them.
+  if (splits > 1) {
+    if (!met) ptx::cluster_wait();     // every thread waits once for the arrival at set-up ...
+    if (!done) ptx::cluster_arrive_relaxed();
+    ptx::cluster_wait();               // ... and once for the others' end
+  }
   __syncthreads();
   const int aborted = *abort_flag;
-  if (splits > 1) ptx::cluster_sync();
   if (aborted != 0) {
     const long long start = clock64();
     while (clock64() - start < (1ll << 22)) {
