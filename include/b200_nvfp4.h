@@ -481,7 +481,8 @@ B200_NVFP4_API long long b200_nvfp4_launch_count(void);
  * A [M, K] and B [N, K]: E4M3 bytes, row-major, K contiguous, 16-byte aligned. a_scale: FP32
  * [M, ceil(K/128)]; b_scale: FP32 [ceil(N/128), ceil(K/128)] (one per 128 x 128 tile, as FP8
  * checkpoints hold them). FP32 sums, one rounding to the output type: out_type 0 = FP16, 1 = FP32,
- * 2 = BF16; C row-major [M, N], 16-byte aligned. M >= 0, N % 8 == 0, K % 16 == 0; M == 0 does nothing.
+ * 2 = BF16; C row-major [M, N], 16-byte aligned. M >= 0, N % 8 == 0, K % 16 == 0, each at most 0x7fffff00; M == 0 does
+ * nothing.
  * A row, scale or code that is NaN or infinite reaches only its own output row (A) or column (B). */
 B200_NVFP4_API int b200_nvfp4_fp8_gemm(int m, int n, int k, const void* a, const void* b, const void* a_scale,
                                        const void* b_scale, void* c, int out_type, b200_stream_t stream);
@@ -489,16 +490,16 @@ B200_NVFP4_API int b200_nvfp4_fp8_gemm(int m, int n, int k, const void* a, const
 /* The same for expert-major rows: group g's rows [cu_seqlens[g], cu_seqlens[g] + seqlens[g]) of x
  * [m, K] (x_scale [m, ceil(K/128)]) times its own weights w [num_group, N, K] (w_scale [num_group,
  * ceil(N/128), ceil(K/128)]). seqlens / cu_seqlens are int32 on the device and never read by the
- * host; ranges may leave gaps, may not
- * overlap, and are cut off where they leave the m rows. Rows of y that belong to no group are left as
- * they were. num_seq_per_group_avg: hint for the tile (0 = m / num_group). num_group <= 1024. */
+ * host; ranges may leave gaps, may not overlap, and are cut off where they leave the m rows. Rows of y that belong to no group are left as
+ * they were. num_seq_per_group_avg: hint for the tile (0 = m / num_group). num_group <= 1024,
+ * num_group * N <= 0x7fffff00. */
 B200_NVFP4_API int b200_nvfp4_fp8_grouped_gemm(void* y, const void* x, const void* w, const void* seqlens,
                                                const void* cu_seqlens, const void* x_scale, const void* w_scale,
                                                int num_group, int m, int n, int k, int num_seq_per_group_avg,
                                                int out_type, b200_stream_t stream);
 
-/* Tile of the FP8 products for tests and tuning, process-wide: rows of A per tile (16 / 32 / 64 / 128
- * with the weights on the MMA's wide side, 512 = 256 x 256 on CTA pairs) and CTAs per tile over K
+/* Tile of the FP8 products for tests and tuning, process-wide: rows of A per tile (16 / 32 / 64 with
+ * the weights on the MMA's 128-row side, 128 with A there, 512 = 256 x 256 on CTA pairs) and CTAs per tile over K
  * (1 / 2 / 4 / 8; not for 512); 0 = built-in rule. */
 B200_NVFP4_API int b200_nvfp4_fp8_set_tile(int tile, int splits);
 
@@ -506,7 +507,8 @@ B200_NVFP4_API int b200_nvfp4_fp8_set_tile(int tile, int splits);
  * scale = RN(amax / 448), q = E4M3(RN(x / scale)). x [rows, K] row-major of input_dtype 0 = FP16, 1 = BF16,
  * 2 = FP32; with swiglu != 0 x is [rows, 2K], gate then up, and silu(gate) * up (each
  * step rounded to FP32) is quantised. q [rows, K] bytes, scale [rows,
- * ceil(K/128)]; x and q 16-byte aligned, K % 16 == 0, rows >= 0. A block that holds a NaN or an
+ * ceil(K/128)]; x and q 16-byte aligned, K % 16 == 0, rows >= 0, less than
+ * 2^31 blocks. A block that holds a NaN or an
  * infinity gets a NaN or infinite scale. What b200_nvfp4_fp8_gemm takes as A and a_scale. */
 B200_NVFP4_API int b200_nvfp4_fp8_quantize_rows(void* q, void* scale, const void* x, int rows, int k, int input_dtype,
                                                 int swiglu, b200_stream_t stream);
@@ -524,7 +526,7 @@ B200_NVFP4_API int b200_nvfp4_fp8_quantize_rows(void* q, void* scale, const void
  *   counts[s, e] = n_se,  slope[s, e] = alpha E n_se / (k T_s^2 S'),  loss = sum_se slope_se sum_t p_te
  * i.e. the mean over sequences of alpha sum_e f_e P_e, f_e = n_e E / (k T_s), P_e = mean_t p_te.
  * loss: one FP32; counts int32 [S, E]; slope FP32 [S, E] (what the backward pass needs). Results do not
- * depend on scheduling. T >= 0, 0 < k <= E <= 4096, 0 < S <= 65536. The workspace (256-byte aligned)
+ * depend on scheduling. 0 <= T <= 2^30, T k < 2^31, 0 < k <= E <= 4096, 0 < S <= 65536. The workspace (256-byte aligned)
  * is scratch for this call alone. */
 B200_NVFP4_API size_t b200_nvfp4_moe_balance_loss_workspace_bytes(int num_tokens, int num_experts, int num_sequences);
 B200_NVFP4_API int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const void* logits,

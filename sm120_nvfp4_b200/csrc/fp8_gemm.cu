@@ -21,6 +21,7 @@ std::atomic<int> g_fp8_tile{0};
 std::atomic<int> g_fp8_splits{0};
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 struct Fp8Problem {
   int groups, rows, n, k;
@@ -206,8 +207,9 @@ int fp8_product(const Fp8Problem& q, const void* a_scale, const void* b_scale, v
 }
 
 bool valid_fp8(int rows, int n, int k, int out_type) {
-  // (row coordinates of a tile that reaches past the end still have to fit 32 bits)
-  return rows >= 0 && rows <= kMaxRows && n > 0 && n <= kMaxRows && k > 0 && (k % 16) == 0 && (n % 8) == 0 && out_type >= kOutF16 && out_type <= kOutBf16;
+  // (coordinates of a tile or block that reaches past the end still have to fit 32 bits)
+  return rows >= 0 && rows <= kMaxRows && n > 0 && n <= kMaxRows && k > 0 && k <= kMaxRows && (k % 16) == 0 && (n % 8) == 0 &&
+         out_type >= kOutF16 && out_type <= kOutBf16;
 }
 
 }  // namespace
@@ -219,7 +221,7 @@ int b200_nvfp4_fp8_gemm(int m, int n, int k, const void* a, const void* b, const
                         int out_type, b200_stream_t stream) {
   using namespace b200;
   if (!valid_fp8(m, n, k, out_type) || a == nullptr || b == nullptr || a_scale == nullptr || b_scale == nullptr ||
-      c == nullptr || !aligned16(a) || !aligned16(b) || !aligned16(c))
+      c == nullptr || !aligned16(a) || !aligned16(b) || !aligned16(c) || !aligned4(a_scale) || !aligned4(b_scale))
     return B200_NVFP4_INVALID_ARGUMENT;
   const Fp8Problem q{1, m, n, k, a, b, nullptr, nullptr, m};
   return fp8_product(q, a_scale, b_scale, c, out_type, static_cast<cudaStream_t>(stream));
@@ -231,7 +233,8 @@ int b200_nvfp4_fp8_grouped_gemm(void* y, const void* x, const void* w, const voi
   using namespace b200;
   if (!valid_fp8(m, n, k, out_type) || num_group <= 0 || num_group > kMaxGroups || y == nullptr || x == nullptr ||
       w == nullptr || seqlens == nullptr || cu_seqlens == nullptr || x_scale == nullptr || w_scale == nullptr ||
-      !aligned16(y) || !aligned16(x) || !aligned16(w) || static_cast<long long>(num_group) * n > kMaxRows)
+      !aligned16(y) || !aligned16(x) || !aligned16(w) || !aligned4(seqlens) || !aligned4(cu_seqlens) || !aligned4(x_scale) ||
+      !aligned4(w_scale) || static_cast<long long>(num_group) * n > kMaxRows)
     return B200_NVFP4_INVALID_ARGUMENT;
   const int avg = num_seq_per_group_avg > 0 ? num_seq_per_group_avg : (m + num_group - 1) / num_group;
   const Fp8Problem q{num_group, m, n, k, x, w, static_cast<const int*>(seqlens), static_cast<const int*>(cu_seqlens), avg};

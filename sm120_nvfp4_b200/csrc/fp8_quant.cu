@@ -213,8 +213,8 @@ extern "C" int b200_nvfp4_fp8_quantize_rows(void* q, void* scale, const void* x,
                                             b200_stream_t stream) {
   using namespace b200;
   const long long kb = (static_cast<long long>(k) + 127) / 128;
-  if (rows < 0 || k <= 0 || (k % 16) != 0 || q == nullptr || scale == nullptr || x == nullptr || !aligned16(q) ||
-      !aligned16(x) || input_dtype < 0 || input_dtype > 2 || rows * kb > 0x7fffffffLL)
+  if (rows < 0 || k <= 0 || k > 0x7fffff00 || (k % 16) != 0 || q == nullptr || scale == nullptr || x == nullptr || !aligned16(q) ||
+      !aligned16(x) || (reinterpret_cast<uintptr_t>(scale) & 3u) != 0 || input_dtype < 0 || input_dtype > 2 || rows * kb > 0x7fffffffLL)
     return B200_NVFP4_INVALID_ARGUMENT;
   const DeviceInfo& dev = current_device_info();
   if (!dev.ok) return B200_NVFP4_CUDA_ERROR;

@@ -18,6 +18,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxExperts = 4096;
 constexpr int kMaxSequences = 65536;
+constexpr int kMaxTokens = 1 << 30;     // token numbers a few steps past the end fit 32 bits; so do counts of slots
 constexpr float kMinSum = 1e-25f;      // below this the sigmoids of a row are e^z to FP32 precision
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -261,7 +262,7 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 inline size_t element_size(int dtype) { return dtype == 2 ? 4 : 2; }
 
 inline bool valid_router(int tokens, int experts, int topk, int sequences, int dtype) {
-  return tokens >= 0 && experts > 0 && experts <= kMaxExperts && topk > 0 && topk <= experts && sequences > 0 &&
+  return tokens >= 0 && tokens <= kMaxTokens && static_cast<long long>(tokens) * topk <= 0x7fffffffLL && experts > 0 && experts <= kMaxExperts && topk > 0 && topk <= experts && sequences > 0 &&
          sequences <= kMaxSequences && dtype >= 0 && dtype <= 2;
 }
 

@@ -300,7 +300,9 @@ int b200_nvfp4_moe_router_backward(void* grad_logits, const void* logits, const 
       (num_tokens > 0 && (grad_logits == nullptr || logits == nullptr || topk_ids == nullptr)) ||
       (grad_weights == nullptr && slope == nullptr) || (grad_weights != nullptr && topk_weights == nullptr) ||
       (slope != nullptr && grad_loss == nullptr) || (cu_seqlens == nullptr && num_sequences != 1) ||
-      !aligned(logits, element_size(logits_dtype)) || !aligned(grad_logits, element_size(logits_dtype)))
+      !aligned(logits, element_size(logits_dtype)) || !aligned(grad_logits, element_size(logits_dtype)) ||
+      !aligned(topk_ids, 4) || !aligned(topk_weights, 4) || !aligned(grad_weights, 4) || !aligned(slope, 4) ||
+      !aligned(grad_loss, 4) || !aligned(cu_seqlens, 4))
     return B200_NVFP4_INVALID_ARGUMENT;
   const DeviceInfo& dev = current_device_info();
   if (!dev.ok) return B200_NVFP4_CUDA_ERROR;

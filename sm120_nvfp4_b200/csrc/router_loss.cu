@@ -363,7 +363,9 @@ int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const voi
   using namespace b200::router;
   if (!valid_router(num_tokens, num_experts, num_topk, num_sequences, logits_dtype) || loss == nullptr || counts == nullptr ||
       slope == nullptr || (num_tokens > 0 && (logits == nullptr || topk_ids == nullptr)) || scoring < 0 || scoring > 1 ||
-      (cu_seqlens == nullptr && num_sequences != 1) || !aligned(logits, element_size(logits_dtype)) || !aligned(workspace, 256))
+      (cu_seqlens == nullptr && num_sequences != 1) || !aligned(logits, element_size(logits_dtype)) ||
+      !aligned(workspace, 256) || !aligned(loss, 4) || !aligned(counts, 4) || !aligned(slope, 4) || !aligned(topk_ids, 4) ||
+      !aligned(cu_seqlens, 4))
     return B200_NVFP4_INVALID_ARGUMENT;
   const LossLayout l = loss_layout(num_tokens, num_experts, num_sequences);
   if (workspace == nullptr || workspace_bytes < l.total) return B200_NVFP4_INSUFFICIENT_WORKSPACE;

@@ -23,7 +23,7 @@ namespace {
 using at::ScalarType;
 using at::Tensor;
 
-constexpr int64_t kMost = 0x7fffff00;
+constexpr int64_t kMost = 0x7fffff00, kMostTokens = 1 << 30;
 
 int64_t blocks_128(int64_t n) { return (n + 127) / 128; }
 
@@ -195,7 +195,7 @@ bool router_args(PyObject* logits, PyObject* ids, PyObject* cu, RouterArgs* r) {
   r->code = input_code(r->logits->scalar_type());
   r->tokens = r->logits->size(0);
   r->experts = r->logits->size(1);
-  if (r->code < 0 || r->tokens <= 0 || r->tokens > kMost || r->experts > 4096 || !on(r->ids, r->index) ||
+  if (r->code < 0 || r->tokens <= 0 || r->tokens > kMostTokens || r->experts > 4096 || !on(r->ids, r->index) ||
       r->ids->scalar_type() != ScalarType::Int || r->ids->dim() != 2 || r->ids->size(0) != r->tokens)
     return false;
   r->topk = r->ids->size(1);
@@ -204,7 +204,7 @@ bool router_args(PyObject* logits, PyObject* ids, PyObject* cu, RouterArgs* r) {
     if (!on(r->cu, r->index) || r->cu->scalar_type() != ScalarType::Int || r->cu->dim() != 1) return false;
     r->sequences = r->cu->numel() - 1;
   }
-  return r->topk > 0 && r->topk <= r->experts && r->sequences > 0 && r->sequences <= 65536;
+  return r->topk > 0 && r->topk <= r->experts && r->tokens * r->topk <= 0x7fffffff && r->sequences > 0 && r->sequences <= 65536;
 }
 
 void* data_or_null(const Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }

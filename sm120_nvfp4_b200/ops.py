@@ -642,6 +642,10 @@ def _on_device(index: int, tensors, names) -> None:
 _FP8_STORAGE = (_FP8, torch.uint8)
 
 
+_FP8_MOST = 0x7fffff00      # rows, columns and K of an FP8 product
+_MOST_TOKENS = 1 << 30
+
+
 def _blocks_128(n: int) -> int:
     return (n + 127) // 128
 
@@ -669,6 +673,8 @@ def quantize_fp8(x: torch.Tensor, *, swiglu: bool = False, output: Optional[torc
         k //= 2
     if not (k > 0 and k % 16 == 0):
         _check(False, "K must be a positive multiple of 16")
+    if not (k <= _FP8_MOST and rows * _blocks_128(k) <= 0x7fffffff):
+        _check(False, "x must hold less than 2^31 blocks of 128 values")
     source = x.data_ptr()
     if not (source % 16 == 0):
         _check(False, "x must be 16-byte aligned")
@@ -707,6 +713,8 @@ def _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output, names):
         _check(False, "K must be a positive multiple of 16")
     if not (n > 0 and n % 8 == 0):
         _check(False, "N must be a positive multiple of 8")
+    if not (max(rows, k, weight.numel() // k) <= _FP8_MOST):
+        _check(False, f"rows, K and the rows of {names[1]} must be at most 0x7fffff00")
     kb = _blocks_128(k)
     if x_scale.shape != (rows, kb):
         _check(False, f"{names[2]} must be [rows, ceil(K/128)]")
@@ -807,6 +815,8 @@ def _check_router(logits, topk_ids, cu_seqlens, scoring):
     k = topk_ids.shape[1]
     if not (0 < k <= e <= 4096):
         _check(False, "need 0 < num_topk <= num_experts <= 4096")
+    if not (t <= _MOST_TOKENS and t * k <= 0x7fffffff):
+        _check(False, "need num_tokens <= 2^30 and fewer than 2^31 slots")
     if not (scoring in _SCORING):
         _check(False, "scoring must be 'sigmoid' or 'softmax'")
     sequences = 1

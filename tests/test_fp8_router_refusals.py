@@ -80,6 +80,59 @@ def test_python_surface_refuses_host_tensors():
             call()
 
 
+def test_sizes_beyond_32_bit_arithmetic_are_refused(L):
+    # K + 127, the fetches a few tokens past the end and counts of slots have to fit 32 bits
+    most = 0x7fffff00
+    assert L.b200_nvfp4_fp8_gemm(1, 8, most + 16, 16, 16, 16, 16, 16, 0, None) == 1
+    assert L.b200_nvfp4_fp8_gemm(most + 1, 8, 16, 16, 16, 16, 16, 16, 0, None) == 1
+    assert L.b200_nvfp4_fp8_grouped_gemm(16, 16, 16, 16, 16, 16, 16, 1, 1, 8, most + 16, 0, 0, None) == 1
+    assert L.b200_nvfp4_fp8_quantize_rows(16, 16, 16, 1, most + 16, 0, 0, None) == 1
+    for t, k in (((1 << 30) + 1, 1), (1 << 30, 2), (1 << 28, 8)):
+        assert L.b200_nvfp4_moe_balance_loss(16, 16, 16, 16, 16, None, t, 8, k, 1, 2, 0, 1.0, 256, 1 << 40, None) == 1
+        assert L.b200_nvfp4_moe_router_backward(16, 16, 16, 16, 16, 16, 16, None, t, 8, k, 1, 2, 0, None) == 1
+    assert L.b200_nvfp4_moe_balance_loss_workspace_bytes((1 << 30) + 1, 8, 1) == 0
+    assert L.b200_nvfp4_moe_balance_loss_workspace_bytes(1 << 30, 8, 1) > 0
+
+
+def test_scales_and_indexes_off_their_alignment_are_refused(L):
+    for i in (5, 6):
+        args = [4, 64, 128, 16, 16, 16, 16, 16, 0, None]
+        args[i] = 18
+        assert L.b200_nvfp4_fp8_gemm(*args) == 1, i
+    for i in (3, 4, 5, 6):
+        args = [16] * 7 + [2, 4, 64, 128, 0, 0, None]
+        args[i] = 18
+        assert L.b200_nvfp4_fp8_grouped_gemm(*args) == 1, i
+    assert L.b200_nvfp4_fp8_quantize_rows(16, 18, 16, 4, 128, 0, 0, None) == 1
+    for i in (0, 1, 2, 4, 5):
+        args = [16] * 6 + [10, 64, 4, 3, 2, 0, 1.0, 256, 1 << 30, None]
+        args[i] = 18
+        assert L.b200_nvfp4_moe_balance_loss(*args) == 1, i
+    for i in (2, 3, 4, 5, 6, 7):
+        args = [16] * 8 + [10, 64, 4, 3, 2, 0, None]
+        args[i] = 18
+        assert L.b200_nvfp4_moe_router_backward(*args) == 1, i
+
+
+@pytest.mark.gpu
+def test_python_surface_refuses_sizes_beyond_the_limits():
+    import sm120_nvfp4_b200 as ops
+    z = torch.empty(((1 << 30) + 1, 1), dtype=torch.float16, device="cuda")
+    ids = torch.empty(((1 << 30) + 1, 1), dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.router_balance_loss(z, ids),
+                 lambda: ops.router_backward(z, ids, slope=torch.zeros((1, 1), device="cuda"), grad_loss=torch.ones((), device="cuda"))):
+        with pytest.raises(RuntimeError, match="2\\^30"):
+            call()
+    a = z.view(torch.uint8)[:0x7fffff10 // 2].view(1, 0x7fffff10)
+    b = torch.empty((8, 0x7fffff10), dtype=torch.uint8, device="cuda")
+    scales = torch.empty((1, (0x7fffff10 + 127) // 128), device="cuda")
+    with pytest.raises(RuntimeError, match="0x7fffff00"):
+        ops.fp8_gemm(a, b, scales, scales)
+    del b
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        ops.quantize_fp8(torch.empty((1, 0x7fffff10), dtype=torch.float16, device="cuda"))
+
+
 @pytest.mark.gpu
 def test_python_surface_refuses_wrong_shapes_and_types():
     import sm120_nvfp4_b200 as ops

@@ -446,3 +446,78 @@ def test_the_long_way_gives_the_same_results(ops, monkeypatch):
     monkeypatch.setattr(_lib, "calls", lambda: _Declines())
     for p, q in zip(short, everything()):
         assert p.dtype == q.dtype and p.shape == q.shape and torch.equal(p.contiguous().view(-1).view(torch.uint8), q.contiguous().view(-1).view(torch.uint8))
+
+
+@pytest.mark.parametrize("tile", [0, 16, 128])
+def test_offsets_beyond_32_bits(ops, L, tile):
+    # A and the output have more than 2^31 elements; only the first and the last rows are not zero
+    m, n, k, ends = (1 << 20) + 5, 2056, 2064, 24
+    a = torch.zeros((m, k), dtype=torch.uint8, device="cuda")
+    sa = torch.ones((m, blocks(k)), device="cuda")
+    b, sb = weight(n, k, 2)
+    x, sx = codes(2 * ends, k, 1)
+    for at, part in ((slice(0, ends), slice(0, ends)), (slice(m - ends, m), slice(ends, 2 * ends))):
+        a[at] = x.view(torch.uint8)[part]
+        sa[at] = sx[part]
+    assert L.b200_nvfp4_fp8_set_tile(tile, 0) == 0
+    out = ops.fp8_gemm(a, b, sa, sb)
+    want, total = reference(x, sx, b, sb)
+    check(torch.cat((out[:ends], out[m - ends:])), want, total, k)
+    assert int(torch.count_nonzero(out[ends:m - ends])) == 0
+
+
+def test_quantiser_offsets_beyond_32_bits(ops):
+    rows, k, ends = (1 << 20) + 5, 2064, 24
+    for swiglu in (False, True):
+        x = torch.zeros((rows, (2 if swiglu else 1) * k), dtype=torch.float16, device="cuda")
+        x[:ends].normal_()
+        x[-ends:].normal_()
+        q, s = ops.quantize_fp8(x, swiglu=swiglu)
+        for at in (slice(0, ends), slice(rows - ends, rows)):
+            wq, ws = ops.quantize_fp8(x[at].contiguous(), swiglu=swiglu)
+            assert torch.equal(s[at], ws) and torch.equal(q[at].view(torch.uint8), wq.view(torch.uint8))
+        assert int(torch.count_nonzero(q[ends:-ends].view(torch.uint8) & 0x7f)) == 0
+        del x, q, s
+
+
+def test_weights_beyond_32_bits(ops, L):
+    groups, n, k = 40, 7168, 8192
+    w = torch.zeros((groups, n, k), dtype=torch.uint8, device="cuda")
+    sw = torch.ones((groups, blocks(n), blocks(k)), device="cuda")
+    last, s_last = weight(n, k, 3)
+    w[-1], sw[-1] = last.view(torch.uint8), s_last
+    x, sx = codes(6, k, 4)
+    n1 = torch.zeros(groups, dtype=torch.int32, device="cuda")
+    n1[0], n1[-1] = 2, 4
+    cu = torch.nn.functional.pad(n1.cumsum(0), (1, 0)).to(torch.int32)
+    want, total = reference(x[2:], sx[2:], last, s_last)
+    for tile in (0, 128, 512):
+        assert L.b200_nvfp4_fp8_set_tile(tile, 0) == 0
+        out = ops.fp8_grouped_gemm(x, w, n1, cu, sx, sw)
+        check(out[2:], want, total, k)
+        assert int(torch.count_nonzero(out[:2])) == 0
+
+
+def test_several_streams_at_once(ops):
+    # every kernel of this file beside the others and beside the four-bit product, whose tensor memory they share
+    g = torch.Generator(device="cuda").manual_seed(7)
+    a, sa = codes(24, 4096, 1)
+    big, sbig = codes(1500, 4096, 2)
+    b, sb = weight(2048, 4096, 3)
+    x = torch.randn((3000, 2048), device="cuda", generator=g)
+    four = [torch.randint(0, 256, (r, 1024), dtype=torch.uint8, device="cuda", generator=g) for r in (300, 1024)]
+    fours = [torch.full((ops.scale_a_elements(300, 1024, 2048),), 0x38, dtype=torch.uint8, device="cuda"),
+             torch.full((ops.scale_b_elements(300, 1024, 2048),), 0x38, dtype=torch.uint8, device="cuda")]
+    calls = [lambda: ops.fp8_gemm(a, b, sa, sb), lambda: ops.fp8_gemm(big, b, sbig, sb), lambda: ops.quantize_fp8(x, swiglu=True)[0],
+             lambda: ops.gemm(*four, *fours)]
+    want = [call().view(torch.uint8) for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(20):
+        for i, call in enumerate(calls):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call())
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        assert all(torch.equal(out.view(torch.uint8), want[i]) for out in outs), i

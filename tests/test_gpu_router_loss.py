@@ -388,3 +388,33 @@ def test_rows_of_any_alignment(ops, t, e, k, offset, dtype):
                               grad_loss=torch.ones((), device="cuda"), cu_seqlens=cu.cuda())
     want, size = reference_grad(z, ids, w, gw, cu, ws, 1.0, "sigmoid", live, seq)
     compare_grad(got, want, size, z)
+
+
+def test_offsets_beyond_32_bits(ops):
+    # logits of more than 2^31 elements: all tokens but the last eight are indifferent between the experts
+    t, e, k, ends = (1 << 19) + 7, 4096, 2, 8
+    gen = torch.Generator().manual_seed(5)
+    z = torch.zeros((t, e), dtype=torch.bfloat16, device="cuda")
+    z[-ends:] = torch.randn((ends, e), generator=gen).to(torch.bfloat16).cuda()
+    ids = (torch.arange(2 * t, dtype=torch.int32, device="cuda") % e).view(t, k)
+    cu = torch.tensor([0, t - 3, t], dtype=torch.int32, device="cuda")
+    loss, counts, slope = ops.router_balance_loss(z, ids, cu_seqlens=cu)
+    want = torch.stack([torch.bincount(ids[:t - 3].flatten().long(), minlength=e), torch.bincount(ids[t - 3:].flatten().long(), minlength=e)])
+    assert torch.equal(counts.long(), want)
+    p = torch.sigmoid(z[-ends:].double())
+    p /= p.sum(1, keepdim=True)
+    tokens = torch.tensor([[t - 3.0], [3.0]], dtype=torch.float64, device="cuda")
+    total = torch.stack([(t - ends) / e + p[:-3].sum(0), p[-3:].sum(0)])
+    exact = float((e * want.double() / (k * tokens ** 2 * 2) * total).sum())
+    # score error as above with |z| < 6, and a chunk's additions: 296 chunks, one thread per column each
+    assert abs(float(loss) - exact) <= exact * ((5 + 1.2 * 6) * 2.0 ** -23 + (t / 290 + 32) * 2.0 ** -24)
+    gw = torch.randn((ends, k), generator=gen).cuda()
+    w = weights_of(z[-ends:].cpu(), ids[-ends:].cpu()).cuda()
+    one = torch.ones((), device="cuda")
+    every_w, every_g = torch.zeros((t, k), device="cuda"), torch.zeros((t, k), device="cuda")
+    every_w[-ends:], every_g[-ends:] = w, gw
+    grad = ops.router_backward(z, ids, topk_weights=every_w, grad_weights=every_g, slope=slope, grad_loss=one, cu_seqlens=cu)
+    near = torch.tensor([0, ends - 3, ends], dtype=torch.int32, device="cuda")
+    part = ops.router_backward(z[-ends:].contiguous(), ids[-ends:].contiguous(), topk_weights=w, grad_weights=gw, slope=slope, grad_loss=one,
+                               cu_seqlens=near)
+    assert torch.equal(grad[-ends:], part)
