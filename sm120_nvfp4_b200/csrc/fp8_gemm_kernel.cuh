@@ -23,6 +23,12 @@
 //                          at 128 rows took longer than everything else (0.75 us per block).
 //                          kWide = true: 128 rows of A on the 128-row side, one scale per thread.
 //   fp8_pair_kernel        many rows: 256 x 256 tiles on CTA pairs (cta_group::2).
+//
+// What bounds them, measured. One row, 4096 x 7168: 8.9 us for 29.4 MB, about 4 us of it start, first loads and
+// end, the rest HBM at 6 TB/s. 77 x 1000 x 1040: 8.8 us, all of it fixed costs and nine dependent blocks. 128 x
+// 4096 x 8192: 16.8 us, the promotion of 16 blocks per CTA (0.38 us each) and the exchange of partial tiles. 64 rows
+// over 32 groups of 4096 x 7168: 125 us, HBM (765 MB, 6.1 TB/s; weights of empty groups are not read). Many
+// rows: see the pair kernel.
 // All waits are bounded (ptx::mbar_wait) and reported through the device error word.
 #pragma once
 
@@ -36,8 +42,8 @@
 namespace b200 {
 
 constexpr int kFp8BlockK = 128;               // values of K per scale = bytes of K per stage row
-constexpr int kFp8Panel = 8;                  // blocks of K whose scales arrive together ...
-constexpr int kFp8Panels = 2;                 // ... and panels in shared memory
+constexpr int kFp8Panel = 8;                  // few rows: blocks of K whose scales arrive together ...
+constexpr int kFp8Panels = 2;                 // ... and panels of them in shared memory
 
 enum Fp8Out { kOutF16 = 0, kOutF32 = 1, kOutBf16 = 2 };
 
@@ -577,6 +583,14 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 // sums. Two such buffers fill the 512 columns of tensor memory. 128 accumulators per thread in eight
 // promotion warps need more registers than an even share (65536 / 384 = 168): the other four warps
 // give theirs up (104 + 2 x 200 = 504 = 3 x 168; 56 / 224 to 104 / 200 differ by what the compiler spills: measured).
+//
+// 8192^3: 480 us in a burst (2290 TFLOP/s), 566 us sustained (1940 TFLOP/s, 0.70 of twice the measured BF16 rate),
+// where power holds the SM clock at 1.46 GHz. The same loads and MMAs with nothing done to their sums take
+// 394 / 466 us, bound by the operands' way from L2 (13.7 TB/s); promotion adds one TMEM read and one FMA per
+// value and block. 4096 x 4096 x 7168 under counters: tensor pipe 60 % of the cycles, FMA pipe 35 %, issue
+// slots 56 %. Tried without gain: MMAs of half the columns (four times as many waits; 527 us), polling
+// barriers between MMAs, packed FMAs (their operands cost moves), loads of the next block before this
+// one's additions (spills: 535 us), a panel of scales read ahead, wider steps than 16 columns.
 struct Fp8PairCfg {
   static constexpr int kThreads = 384;
   static constexpr int kBuffers = 2;

@@ -103,24 +103,19 @@ __device__ __forceinline__ float nvfp4_silu_in_range(float x) {
 
 constexpr float kSiluInRangeLimit = 87.0f;
 
-// v[i] = silu(g[i]) * u[i] for N values: the branch-free form, and the plain one where a gate value
-// lies outside its range (or is an infinity).
-template <int N>
-__device__ __forceinline__ void silu_mul_block(const float (&g)[N], const float (&u)[N], float (&v)[N]) {
+// v[i] = silu(g[i]) * u[i] for one block of 16: the branch-free form, and the plain one for a
+// block that holds a gate value outside its range (or an infinity).
+__device__ __forceinline__ void silu_mul_block16(const float (&g)[16], const float (&u)[16], float (&v)[16]) {
   float gmax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < 16; ++i) {
     gmax = fmaxf(gmax, fabsf(g[i]));
     v[i] = __fmul_rn(nvfp4_silu_in_range(g[i]), u[i]);
   }
   if (gmax > kSiluInRangeLimit) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __fmul_rn(nvfp4_silu(g[i]), u[i]);
+    for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(nvfp4_silu(g[i]), u[i]);
   }
-}
-
-__device__ __forceinline__ void silu_mul_block16(const float (&g)[16], const float (&u)[16], float (&v)[16]) {
-  silu_mul_block(g, u, v);
 }
 
 // Quantises 16 FP32 values: returns the UE4M3 scale code, writes 8 payload bytes as two

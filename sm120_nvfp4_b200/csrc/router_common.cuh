@@ -43,8 +43,7 @@ struct alignas(sizeof(T) * V) Vec {
 // G threads share the row of a token: 8, 16 or 32 lanes of a warp, which then works on 32 / G tokens at
 // a time, or a whole block (256). What a token costs beside its elements - ids, votes, exchanges - is
 // issued once per warp, so narrow groups with 8 to 20 columns per thread beat one warp per token
-// (131072 x 160 BF16 gradient, instructions per token: 433 with a warp, two exponentials per slot and
-// match instructions).
+// (131072 x 160 BF16: loss 62 us with a warp per token, 46 with groups; gradient 91 and 53).
 template <int G>
 struct Group {
   static constexpr int kPerWarp = G >= 32 ? 1 : 32 / G;

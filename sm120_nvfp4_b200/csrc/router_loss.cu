@@ -11,6 +11,10 @@
 // threads keeps a token's row in registers and the sums over its tokens too; partial sums of a block
 // of tokens are written out and added by a second kernel in a fixed order, so that results do not depend
 // on scheduling. Counts are whole numbers and may be added in any order.
+//
+// 65536 x 256 FP32: 27 us where the bytes take 10.6. The first kernel (20 us) is bound by the special-function unit -
+// an exponential and a reciprocal per logit, sixteen a cycle per SM - with half of the issue slots
+// used; the second is 7 us of latencies, of which its early start hides a part. 131072 x 160 BF16: 29 us.
 #include "router_common.cuh"
 
 namespace b200 {
@@ -290,8 +294,8 @@ balance_reduce_kernel(const LossParams p) {
 
 // Tokens per work item. Two blocks of the first kernel are resident per SM, and there are about as many
 // items as chunks and sequences together: with few sequences the items fill the GPU exactly once (a
-// few items more than that cost a second round: 467 items on 444 places took 43 us where 296 take
-// half), with many sequences there are several rounds anyway. Fixed, so that the order of the sums does
+// few items more than that cost a second round: 131072 x 160 BF16 46 us with 467 items on 444 places, 40
+// with 296), with many sequences there are several rounds anyway. Fixed, so that the order of the sums does
 // not depend on the device: 148 SMs.
 int loss_chunk(int tokens, int sequences) {
   constexpr int kResident = 2 * 148;

@@ -5,7 +5,7 @@
 // the outputs and calls the C ABI on torch's current stream of the tensors' device. Where anything is
 // not as the usual call has it - a wrong type, shape, device or alignment, no rows - it does nothing and
 // returns None; the Python function then goes its own, complete way, which says what is wrong. One call of
-// fp8_gemm for one row costs 5 us of host time this way, 10.5 through ctypes.
+// fp8_gemm for one row costs 4.9 us of host time this way, 10.5 through ctypes.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
