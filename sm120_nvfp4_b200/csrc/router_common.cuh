@@ -35,6 +35,14 @@ __device__ __forceinline__ float reciprocal(float x) {
   return r;
 }
 
+// e^x = 2^(x log2 e) by the exponential instruction: off by 2 + 1.173 |x| units of 2^-23 at most; results below
+// 2^-126 are 0. (__expf keeps those, with three more instructions per value.)
+__device__ __forceinline__ float exponential(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
@@ -147,6 +155,12 @@ struct RowQueue {
       for (int j = 0; j < V; ++j) z[i * V + j] = to_float(w.v[j]);
     }
   }
+  // one column of that row, whichever thread has copied it (after a Group::sync())
+  __device__ __forceinline__ float at(int stage, const T*, int col, int lane) const {
+    const int part = col / V;
+    const uint8_t* from = mine + stage * kStage + (part / G * kThreads + part % G - lane) * static_cast<int>(sizeof(Part));
+    return to_float(reinterpret_cast<const Part*>(from)->v[col % V]);
+  }
 };
 
 // 16-bit rows that cannot be copied by the column (asynchronous copies have 4 bytes at least): the group
@@ -189,6 +203,9 @@ struct RowQueue<T, 1, NV, G, true> {
     }
     Group<G>::sync();                                       // before the place is filled again
   }
+  __device__ __forceinline__ float at(int stage, const T* row, int col, int) const {
+    return to_float(reinterpret_cast<const T*>(mine + stage * kRow + (reinterpret_cast<uintptr_t>(row) & 15))[col]);
+  }
 };
 
 // A queue of one 4-byte word per thread and step.
@@ -217,7 +234,7 @@ __device__ __forceinline__ float exponentials(float (&z)[N], float* scratch) {
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    z[i] = z[i] == __int_as_float(0xff800000) ? 0.0f : __expf(z[i] - top);
+    z[i] = z[i] == __int_as_float(0xff800000) ? 0.0f : exponential(z[i] - top);
     sum += z[i];
   }
   sum = Group<G>::sum(sum, scratch);

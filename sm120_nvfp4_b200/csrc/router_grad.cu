@@ -3,8 +3,9 @@
 // forward pass; the counts are constants):
 //   loss      dz_e  = g p_e (1 - s_e) (slope_e - sum_j slope_j p_j)       (softmax: without 1 - s)
 //   weights   dz_j += w_j (1 - s_j) (g_j - sum_i g_i w_i)                 for each selected expert j,
-// the second from w_j = s_j / (sum of the selected s). What the weights add waits, without its factor
-// 1 - s, at the selected columns of a row in shared memory; the thread that holds a column merges it.
+// the second from w_j = s_j / (sum of the selected s). The threads that hold a token's slots work out what
+// the weights add and lay it at the selected columns of a row in shared memory, zero elsewhere; the
+// threads that hold the columns add it.
 //
 // Reads the logits, ids, weights and their gradient once and writes the gradient: 8 E + 12 k bytes per
 // token of FP32 logits. 131072 x 160 BF16: 35.6 us where the bytes take 14.2; 65536 x 256 FP32: 31 us (21). Bound by
@@ -27,13 +28,6 @@ struct GradParams {
   int chunk;                  // consecutive tokens per group of threads
   int softmax;
 };
-
-// minimum that keeps a NaN
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 template <typename T, int V, int NV, int G>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -152,26 +146,27 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
     const bool inside = Gr::any(mine) && in && through_loss && t >= s_begin && t < s_end;
     t += Gr::kPerWarp;
 
-    // s = 1 / (1 + u), 1 - s = u s with u = e^-z, held below 2^126 so that neither overflows. What is kept
-    // is s (1 - s) in `both`, which the gradient of the loss has as a factor, and 1 - s.
-    float both[N], rest[N];
-    float sum = 0.0f, dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float u = __expf(min_nan(-z[i], 87.0f));
-      const float x = reciprocal(1.0f + u);
-      rest[i] = u * x;
-      const float sc = z[i] <= -87.0f ? 0.0f : x;
-      both[i] = sc * rest[i];
-      sum += sc;
-      dot = fmaf(d[i], sc, dot);
-    }
+    float out_row[N];                                      // s (1 - s), then the gradient
     if (through_loss) {
-      sum = Gr::sum(sum, scratch);
-      dot = Gr::sum(dot, scratch);
+      float sum = 0.0f, dot = 0.0f;
+      if (!p.softmax) {
+        // with w = e^-|z|: the larger of s and 1 - s is r = 1 / (1 + w), the smaller w r
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float w = exponential(-fabsf(z[i]));
+          const float r = reciprocal(1.0f + w);
+          const float wr = w * r;
+          out_row[i] = wr * r;
+          const float sc = z[i] < 0.0f ? wr : r;
+          sum += sc;
+          dot = fmaf(d[i], sc, dot);
+        }
+        sum = Gr::sum(sum, scratch);
+        dot = Gr::sum(dot, scratch);
+      }
       const bool by_max = inside && (p.softmax || !(sum >= kMinSum));
       float inv = reciprocal(sum);
-      if (Gr::any_here(by_max)) {      // softmax, or scores that all vanish: they are e^z then
+      if (Gr::any_here(by_max)) {      // softmax, or scores that all vanish: they are e^z then, and 1 - s is 1
         const float other = exponentials<N, G>(z, scratch);
         float dot2 = 0.0f;
 #pragma unroll
@@ -180,19 +175,19 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         inv = by_max ? other : inv;
         dot = by_max ? dot2 : dot;
 #pragma unroll
-        for (int i = 0; i < N; ++i) both[i] = by_max ? (p.softmax ? z[i] : z[i] * rest[i]) : both[i];
+        for (int i = 0; i < N; ++i) out_row[i] = by_max ? z[i] : out_row[i];
       }
       // g p (1 - s) (slope - dot) with the row's constants multiplied out
       const float by = g * inv, minus = -by * (dot * inv);
 #pragma unroll
-      for (int i = 0; i < N; ++i) z[i] = both[i] * fmaf(by, d[i], minus);
+      for (int i = 0; i < N; ++i) out_row[i] *= fmaf(by, d[i], minus);
       if (Gr::any_here(!inside)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = inside ? z[i] : 0.0f;
+        for (int i = 0; i < N; ++i) out_row[i] = inside ? out_row[i] : 0.0f;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) z[i] = 0.0f;
+      for (int i = 0; i < N; ++i) out_row[i] = 0.0f;
     }
     if (through_weights) {
       if constexpr (G > 32) {
@@ -216,11 +211,14 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         }
         Gr::sync();
       };
-      place(id, w * (gw - mean), min(G, p.topk));
+      // 1 - s of a selected column
+      auto rest = [&](int col) { return reciprocal(1.0f + exponential(rows.at(stage, row, col, lane))); };
+      Gr::sync();
+      place(id, id >= 0 ? w * (gw - mean) * rest(id) : 0.0f, min(G, p.topk));
       for (int j0 = G; j0 < p.topk; j0 += G) {
         int to = in && j0 + lane < p.topk ? p.ids[slots + j0 + lane] : -1;
         if (static_cast<unsigned>(to) >= static_cast<unsigned>(p.experts)) to = -1;
-        place(to, to >= 0 ? p.weights[slots + j0 + lane] * (p.grad_weights[slots + j0 + lane] - mean) : 0.0f, min(G, p.topk - j0));
+        place(to, to >= 0 ? p.weights[slots + j0 + lane] * (p.grad_weights[slots + j0 + lane] - mean) * rest(to) : 0.0f, min(G, p.topk - j0));
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -228,8 +226,7 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         if (col < p.experts) {
           const Vec<float, V> x = *reinterpret_cast<const Vec<float, V>*>(add + col);
 #pragma unroll
-          for (int j = 0; j < V; ++j)      // (a NaN logit that was not selected must not reach its column)
-            if (x.v[j] != 0.0f) z[i * V + j] = fmaf(rest[i * V + j], x.v[j], z[i * V + j]);
+          for (int j = 0; j < V; ++j) out_row[i * V + j] += x.v[j];
         }
       }
       Gr::sync();
@@ -249,7 +246,7 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
         if (col < p.experts) {
           Vec<T, V> x;
 #pragma unroll
-          for (int j = 0; j < V; ++j) from_float(z[i * V + j], &x.v[j]);
+          for (int j = 0; j < V; ++j) from_float(out_row[i * V + j], &x.v[j]);
           *reinterpret_cast<Vec<T, V>*>(out + col) = x;
         }
       }

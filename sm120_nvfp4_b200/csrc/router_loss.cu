@@ -143,35 +143,34 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
     const bool live = Gr::any(mine);
     if (!Gr::any_here(live)) continue;
     live_tokens += live;
-    float inv = -1.0f;
+    auto add = [&](const float (&x)[N], float inv) {
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
+      }
+    };
     if (!p.softmax) {
-      // 1 / (1 + e^-z) from __expf and the reciprocal instruction: a few ulp
+      // 1 / (1 + e^-z) from the exponential and the reciprocal instruction: a few ulp
       float sc[N];
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        sc[i] = reciprocal(1.0f + __expf(-z[i]));
+        sc[i] = reciprocal(1.0f + exponential(-z[i]));
         sum += sc[i];
       }
       sum = Gr::sum(sum, scratch);
       const bool vanish = live && !(sum >= kMinSum);
+      float inv = reciprocal(sum);
       if (Gr::any_here(vanish)) {
         // scores that all vanish (every logit below about -57) are e^z: normalised as e^(z - max)
         const float other = exponentials<N, G>(z, scratch);
-        inv = vanish ? other : __fdividef(1.0f, sum);
+        inv = vanish ? other : inv;
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = vanish ? z[i] : sc[i];
-      } else {
-        inv = __fdividef(1.0f, sum);
-#pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = sc[i];
+        for (int i = 0; i < N; ++i) sc[i] = vanish ? z[i] : sc[i];
       }
+      add(sc, inv);
     } else {
-      inv = exponentials<N, G>(z, scratch);
-    }
-    if (live) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = fmaf(z[i], inv, acc[i]);
+      add(z, exponentials<N, G>(z, scratch));
     }
   }
   if (lane == 0) atomicAdd(&s_live, live_tokens);
