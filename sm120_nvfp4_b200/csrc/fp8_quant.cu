@@ -5,9 +5,9 @@
 //
 // Reads 2 bytes (4 with SiLU) and writes 1.03 per value of a 16-bit input. Eight (or sixteen) lanes share a
 // block: 16-byte loads, an amax by three (four) exchanges, one 16-byte (8-byte) store. 32768 x 4096 BF16:
-// 71 us, 0.87 of what the bytes take at the measured copy rate. 32768 x 2048 with SiLU: 84 us, 0.61 of it, bound by
-// instruction issue (81 % of the slots; 35 instructions per value, most of them the exponential and
-// the IEEE division of the SiLU, which keep it equal to the plain FP32 formula to the bit).
+// 71 us, 0.87 of what the bytes take at the measured copy rate. 32768 x 2048 with SiLU: 68 us, 0.76 of it: 25
+// instructions per value, half of them the exponential and the division of the SiLU, at 66 % of the issue
+// slots, and the wait for the loads.
 //
 // The division: every quotient of a block has the same divisor s, so one correctly rounded reciprocal
 // r = RN(1 / s) serves them all by Markstein's sequence (IBM J. Res. Dev. 34(1), 1990): q0 = RN(x r),
@@ -33,6 +33,13 @@ constexpr float kAmaxFloor = 8.67361737988403547e-19f;   // 2^-60
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 1 / x to one unit in the last place, x normal.
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -113,17 +120,36 @@ __device__ __forceinline__ void minus_quotients(float (&v)[N], float s, float y)
   }
 }
 
-// silu(g) * u = g / (1 + e^-g) * u in IEEE FP32 steps.
+// silu(g) * u = g / (1 + e^-g) * u. The quotient is Markstein's sequence again, here on the reciprocal
+// instruction, which is one unit off at most: the corrected quotient is off by half a unit and 2^-21 of one
+// at most, so it is the IEEE division's but for one value in some 2^20 (none in 2^27 random ones; 80 -> 72 us). It is computed with its sign turned
+// round for the sake of zeros, as above, and -u turns it back. Gates beyond 87, whose divisor or remainder could
+// leave the range, send the thread's values through IEEE divisions (the divisor is below 2^126 otherwise).
 template <int N>
 __device__ __forceinline__ void silu_mul(float (&v)[N], const float (&u)[N]) {
+  float top = 0.0f;
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = __fmul_rn(__fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))), u[j]);
+  for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(v[j]));
+  if (top <= 87.0f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = 1.0f + expf(-v[j]);
+      const float y = -reciprocal(d);
+      const float q0 = __fmul_rn(v[j], y);
+      v[j] = __fmul_rn(__fmaf_rn(__fmaf_rn(q0, d, v[j]), y, q0), -u[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __fmul_rn(__fdiv_rn(v[j], __fadd_rn(1.0f, expf(-v[j]))), u[j]);
+  }
 }
 
+// Five blocks per SM, 48 registers, for 16-bit types: 32768 x 2048 with SiLU 71.8 -> 67.6 us; FP32 does better with
+// the registers it wants (16384 x 2048 with SiLU 46.3, 49.4 held to 48).
 // kPer values per thread: 128 / kPer lanes share a block of 128. `step_rows`, `step_cols`: how far the next of a
 // thread's kUnroll blocks is, in rows and blocks (the blocks a thread block handles at a time / kb, % kb).
 template <typename T, bool kSwiglu, int kPer, int kUnroll>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, kPer == 16 ? 5 : 0)
 fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T* __restrict__ x, int k, uint32_t kb,
                     uint32_t blocks, uint32_t step_rows, uint32_t step_cols) {
   constexpr int kLanes = 128 / kPer;
@@ -197,7 +223,7 @@ void launch_quantize(void* q, void* scale, const void* x, int k, uint32_t kb, ui
   // where that leaves SMs idle, and for FP32, whose loads would be strided further apart (16384 x 4096: 53.4
   // us with sixteen and one block, 51.3 with eight and two). More blocks per thread cost more
   // occupancy than their overlapped loads bring: 32768 x 4096 BF16 74 us with one, 86 with two; with SiLU
-  // 32768 x 2048 88 and 109.
+  // 32768 x 2048 88 and 109 (both before later steps).
   constexpr int kPer = sizeof(T) == 2 ? 16 : 8;
   constexpr int kUnroll = sizeof(T) == 4 && !kSwiglu ? 2 : 1;
   if (blocks >= static_cast<uint32_t>(sms) * 2u * 2u * kPer * kUnroll)

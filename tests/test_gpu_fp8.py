@@ -307,6 +307,31 @@ def test_quantiser_with_silu(ops, dtype, rows, k):
     assert ((q.cpu().double() - u).abs() <= step * (1 + 2.0 ** -19) + 16 * 2.0 ** -24 * u.abs()).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantiser_with_silu_of_special_values(ops, dtype):
+    # one special pair per block: zeros of both signs, gates around and beyond +-87, tiny ones, infinities, NaN
+    tiny = float(torch.finfo(dtype).tiny)
+    gates = [0.0, -0.0, 86.5, -86.5, 87.5, -87.5, 100.0, -100.0, tiny, -tiny, float("inf"), float("-inf"), float("nan"), 1.0]
+    ups = [1.0, -1.0, 0.0, -0.0, 1000.0, float("inf"), float("nan")]
+    pairs = [(a, b) for a in gates for b in ups]
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((len(pairs), 256), generator=g).to(dtype)
+    x[:, 5], x[:, 128 + 5] = torch.tensor([a for a, _ in pairs]).to(dtype), torch.tensor([b for _, b in pairs]).to(dtype)
+    q, s = ops.quantize_fp8(x.cuda(), swiglu=True)
+    gate, up = x[:, :128].double(), x[:, 128:].double()
+    v = gate / (1.0 + torch.exp(-gate)) * up
+    finite = torch.isfinite(v).all(1)
+    assert torch.equal(torch.isfinite(s.cpu()[:, 0]), finite)
+    v, q, s = v[finite], q.cpu()[finite], s.cpu()[finite]
+    scale = v.abs().amax(1, keepdim=True).clamp(min=2.0 ** -60) / 448.0
+    assert ((s.double() - scale).abs() <= 8 * 2.0 ** -24 * scale).all()
+    u = v / scale
+    step = torch.clamp(u.abs() * 2.0 ** -4, min=2.0 ** -10)
+    assert ((q.double() - u).abs() <= step * (1 + 2.0 ** -19) + 16 * 2.0 ** -24 * u.abs()).all()
+    zero = v == 0
+    assert torch.equal(torch.signbit(q.float())[zero], torch.signbit(v)[zero])
+
+
 # ------------------------------------------------------------------------- as a user's program runs
 
 
