@@ -81,22 +81,8 @@ int launch_skinny(const Fp8Problem& q, Fp8Params p, int splits, const DeviceInfo
   p.raster_m = 16;
   const long long tasks = row_tiles(q, Cfg::kTileM) * ((q.n + Cfg::kTileN - 1) / Cfg::kTileN);
   const long long blocks = splits > 1 ? tasks * splits : (tasks < dev.sm_count ? tasks : dev.sm_count);
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks));
-  config.blockDim = dim3(Cfg::kThreads);
-  config.dynamicSmemBytes = static_cast<size_t>(Cfg::smem_bytes(q.groups, splits));
-  config.stream = stream;
-  cudaLaunchAttribute attrs[1];
-  attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim.x = static_cast<unsigned>(splits);
-  attrs[0].val.clusterDim.y = 1;
-  attrs[0].val.clusterDim.z = 1;
-  config.attrs = attrs;
-  config.numAttrs = splits > 1 ? 1 : 0;
-  const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, tmap_x, tmap_w, p);
-  count_launch();
-  const int status = launch_status();
-  return launched == cudaSuccess ? status : B200_NVFP4_CUDA_ERROR;
+  return launch_overlapped(kernel, static_cast<unsigned>(blocks < 1 ? 1 : blocks), Cfg::kThreads, static_cast<size_t>(Cfg::smem_bytes(q.groups, splits)),
+                           splits, stream, tmap_x, tmap_w, p);
 }
 
 int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStream_t stream) {
@@ -132,9 +118,8 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
   long long pairs = row_tiles(q, 256) * ((q.n + 255) / 256);
   if (pairs > max_pairs[dev.device]) pairs = max_pairs[dev.device];
   if (pairs < 1) pairs = 1;
-  fp8_pair_kernel<<<static_cast<unsigned>(2 * pairs), Cfg::kThreads, Cfg::smem_bytes(q.groups), stream>>>(tmap_a, tmap_b, tmap_out, p);
-  count_launch();
-  return launch_status();
+  return launch_overlapped(fp8_pair_kernel, static_cast<unsigned>(2 * pairs), Cfg::kThreads, static_cast<size_t>(Cfg::smem_bytes(q.groups)), 1, stream,
+                           tmap_a, tmap_b, tmap_out, p);       // (clusters of two by the kernel's own declaration)
 }
 
 // CTAs per tile over K: as many as still fit the GPU at once and leave each enough blocks of K to pay for the

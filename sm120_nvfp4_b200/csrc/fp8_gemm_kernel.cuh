@@ -237,6 +237,8 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     ptx::prefetch_tensormap(kWide ? &tmap_w : &tmap_x);
   }
   ptx::tc_fence_before_sync();
+  ptx::grid_wait();
+  ptx::grid_launch_dependents();
   if (one_group) {
     // the loaders need the barriers only, and start before tensor memory has been allocated
     if (warp == kLoadWide || warp == kLoadNarrow) {
@@ -674,6 +676,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     ptx::prefetch_tensormap(&tmap_out);
   }
   ptx::tc_fence_before_sync();
+  ptx::grid_wait();
+  ptx::grid_launch_dependents();
   fp8_group_tables(p, 256, s_cu_tiles, s_row0, s_rows);
   ptx::cluster_arrive_relaxed();
   ptx::cluster_wait();                        // the partner's barriers exist

@@ -23,6 +23,7 @@
 
 #include "host_common.hpp"
 #include "internal.hpp"
+#include "ptx.cuh"
 
 namespace b200 {
 namespace {
@@ -154,6 +155,8 @@ fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T*
                     uint32_t blocks, uint32_t step_rows, uint32_t step_cols) {
   constexpr int kLanes = 128 / kPer;
   constexpr uint32_t kAtOnce = 256 / kLanes;
+  ptx::grid_wait();
+  ptx::grid_launch_dependents();
   const int lane = threadIdx.x & (kLanes - 1);
   const uint32_t first = blockIdx.x * (kAtOnce * kUnroll) + threadIdx.x / kLanes;
   float v[kUnroll][kPer];
@@ -211,14 +214,15 @@ fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T*
 }
 
 template <typename T, bool kSwiglu, int kPer, int kUnroll>
-void launch_blocks(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, cudaStream_t stream) {
+int launch_blocks(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, cudaStream_t stream) {
   constexpr uint32_t kAtOnce = 256u * kPer / 128u, kPerBlock = kAtOnce * kUnroll;
-  fp8_quantize_kernel<T, kSwiglu, kPer, kUnroll><<<(blocks + kPerBlock - 1) / kPerBlock, 256, 0, stream>>>(
-      static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks, kAtOnce / kb, kAtOnce % kb);
+  return launch_overlapped(fp8_quantize_kernel<T, kSwiglu, kPer, kUnroll>, (blocks + kPerBlock - 1) / kPerBlock, 256, 0, 1, stream,
+                           static_cast<uint8_t*>(q), static_cast<float*>(scale), static_cast<const T*>(x), k, kb, blocks, kAtOnce / kb,
+                           kAtOnce % kb);
 }
 
 template <typename T, bool kSwiglu>
-void launch_quantize(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, int sms, cudaStream_t stream) {
+int launch_quantize(void* q, void* scale, const void* x, int k, uint32_t kb, uint32_t blocks, int sms, cudaStream_t stream) {
   // Sixteen values per thread halve what a block costs beside its values (index, exchanges, scale); eight
   // where that leaves SMs idle, and for FP32, whose loads would be strided further apart (16384 x 4096: 53.4
   // us with sixteen and one block, 51.3 with eight and two). More blocks per thread cost more
@@ -227,9 +231,8 @@ void launch_quantize(void* q, void* scale, const void* x, int k, uint32_t kb, ui
   constexpr int kPer = sizeof(T) == 2 ? 16 : 8;
   constexpr int kUnroll = sizeof(T) == 4 && !kSwiglu ? 2 : 1;
   if (blocks >= static_cast<uint32_t>(sms) * 2u * 2u * kPer * kUnroll)
-    launch_blocks<T, kSwiglu, kPer, kUnroll>(q, scale, x, k, kb, blocks, stream);
-  else
-    launch_blocks<T, kSwiglu, 8, 1>(q, scale, x, k, kb, blocks, stream);
+    return launch_blocks<T, kSwiglu, kPer, kUnroll>(q, scale, x, k, kb, blocks, stream);
+  return launch_blocks<T, kSwiglu, 8, 1>(q, scale, x, k, kb, blocks, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -252,13 +255,11 @@ extern "C" int b200_nvfp4_fp8_quantize_rows(void* q, void* scale, const void* x,
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint32_t kbu = static_cast<uint32_t>(kb);
   switch (input_dtype * 2 + (swiglu != 0)) {
-    case 0: launch_quantize<__half, false>(q, scale, x, k, kbu, blocks, dev.sm_count, s); break;
-    case 1: launch_quantize<__half, true>(q, scale, x, k, kbu, blocks, dev.sm_count, s); break;
-    case 2: launch_quantize<__nv_bfloat16, false>(q, scale, x, k, kbu, blocks, dev.sm_count, s); break;
-    case 3: launch_quantize<__nv_bfloat16, true>(q, scale, x, k, kbu, blocks, dev.sm_count, s); break;
-    case 4: launch_quantize<float, false>(q, scale, x, k, kbu, blocks, dev.sm_count, s); break;
-    default: launch_quantize<float, true>(q, scale, x, k, kbu, blocks, dev.sm_count, s); break;
+    case 0: return launch_quantize<__half, false>(q, scale, x, k, kbu, blocks, dev.sm_count, s);
+    case 1: return launch_quantize<__half, true>(q, scale, x, k, kbu, blocks, dev.sm_count, s);
+    case 2: return launch_quantize<__nv_bfloat16, false>(q, scale, x, k, kbu, blocks, dev.sm_count, s);
+    case 3: return launch_quantize<__nv_bfloat16, true>(q, scale, x, k, kbu, blocks, dev.sm_count, s);
+    case 4: return launch_quantize<float, false>(q, scale, x, k, kbu, blocks, dev.sm_count, s);
+    default: return launch_quantize<float, true>(q, scale, x, k, kbu, blocks, dev.sm_count, s);
   }
-  count_launch();
-  return launch_status();
 }

@@ -17,6 +17,34 @@ inline void count_launch(int n = 1) { g_launch_count.fetch_add(n, std::memory_or
 // fail the next, unrelated call.
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : 6; }
 
+#ifdef __CUDACC__
+// Launch that may start while the kernel before it in the stream drains (programmatic stream serialization):
+// its blocks set themselves up meanwhile, and wait for that kernel's end themselves (ptx::grid_wait) before
+// they touch global memory. `cluster` CTAs to a cluster where it is above 1.
+template <typename... Params, typename... Args>
+int launch_overlapped(void (*kernel)(Params...), dim3 blocks, int threads, size_t smem, int cluster, cudaStream_t stream,
+                      Args... args) {
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = blocks;
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attrs;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, args...);
+  count_launch();
+  const int status = launch_status();
+  return launched == cudaSuccess ? status : 6;
+}
+#endif
+
 int gemm_dense(int groups, int m, int n, int k, const void* a, const void* b, const void* sfa,
                const void* sfb, void* c, bool out_f32, cudaStream_t stream);
 

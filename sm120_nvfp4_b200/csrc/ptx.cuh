@@ -441,6 +441,15 @@ __device__ __forceinline__ void cp_async_mbar_arrive(uint32_t bar) {
 
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// ------------------------------------------------------- overlapped launches
+
+// A kernel launched with programmatic stream serialization may start while the one before it in its stream
+// drains. grid_wait() returns once that one has finished and its writes can be seen: every thread calls
+// it before it touches global memory, and before any wait whose time is limited.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The next kernel of the stream may be started where places are free (it waits for this one's end itself).
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 // ------------------------------------------------------------------ clusters
 
 __device__ __forceinline__ uint32_t cluster_cta_rank() {

@@ -10,6 +10,7 @@
 
 #include "host_common.hpp"
 #include "internal.hpp"
+#include "ptx.cuh"
 
 namespace b200 {
 namespace router {

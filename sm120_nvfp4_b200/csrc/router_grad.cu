@@ -47,6 +47,8 @@ router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const Gra
   int* owner = reinterpret_cast<int*>(add + p.width);
   for (int e = lane; e < p.width; e += G) add[e] = 0.0f;
   Gr::sync();
+  ptx::grid_wait();
+  ptx::grid_launch_dependents();
   // a warp (a block for G > 32) takes `chunk` consecutive tokens, its groups neighbouring ones
   const long long worker = G > 32 ? blockIdx.x : static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int begin = static_cast<int>(min(worker * p.chunk, static_cast<long long>(p.tokens)));
@@ -276,9 +278,7 @@ struct GradLaunch {
     p.chunk = static_cast<int>((chunk + Gr::kPerWarp - 1) / Gr::kPerWarp * Gr::kPerWarp);
     const long long needed = (static_cast<long long>(p.tokens) + p.chunk - 1) / p.chunk;
     const int blocks = static_cast<int>(G > 32 ? needed : (needed + kWarps - 1) / kWarps);
-    kernel<<<blocks, kThreads, smem, stream>>>(static_cast<T*>(grad), static_cast<const T*>(logits), p);
-    count_launch();
-    return launch_status();
+    return launch_overlapped(kernel, blocks, kThreads, smem, 1, stream, static_cast<T*>(grad), static_cast<const T*>(logits), p);
   }
 };
 

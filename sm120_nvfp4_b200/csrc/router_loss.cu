@@ -81,8 +81,9 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
   WordQueue<int> first_ids(s_raw + Rows::kBytes);
   int* s_counts = reinterpret_cast<int*>(s_raw + p.counts_at);
   const int item = blockIdx.x;
+  ptx::grid_wait();
+  ptx::grid_launch_dependents();                           // the second kernel's blocks may take their places
   if (item == 0 && threadIdx.x == 0) *p.ticket = 0;
-  asm volatile("griddepcontrol.launch_dependents;");       // the second kernel's blocks may take their places
   const int s = item_sequence(p, item), c = item - s;
   int lo = 0, hi = 0;
   if (s < p.sequences && c < p.chunks) {
@@ -197,7 +198,8 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
 // One block per sequence and 64 columns: adds the sequence's partial rows (item order within sixteen
 // interleaved strands, then the strands), and the last block to finish adds up the loss. It is a chain of
 // latencies, so everything that does not depend on the partial sums happens before the first kernel's
-// end is waited for, and independent loads are issued together.
+// end is waited for (whatever ran before that kernel has ended: it lets this one start only then), and
+// independent loads are issued together.
 __global__ void __launch_bounds__(kThreads)
 balance_reduce_kernel(const LossParams p) {
   extern __shared__ unsigned s_filled[];                   // one bit per sequence
@@ -216,7 +218,8 @@ balance_reduce_kernel(const LossParams p) {
   const int strand = threadIdx.x >> 4, quad = threadIdx.x & 15;
   const int col = col_block * 64 + quad * 4;
   __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial sums are complete
+  ptx::grid_wait();                                        // the partial sums are complete
+  ptx::grid_launch_dependents();
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   int4 num = make_int4(0, 0, 0, 0);
   if (hi > lo && col < p.width) {
@@ -339,9 +342,8 @@ struct LossLaunch {
     const int allowed = allow_smem(kernel, once, status, device, static_cast<int>(kCountsAt + kMaxWidth * 4));
     if (allowed != B200_NVFP4_SUCCESS) return allowed;
     p.counts_at = static_cast<int>(kCountsAt);
-    kernel<<<p.chunks + p.sequences, kThreads, kCountsAt + static_cast<size_t>(p.width) * 4, stream>>>(static_cast<const T*>(logits), p);
-    count_launch();
-    return launch_status();
+    return launch_overlapped(kernel, p.chunks + p.sequences, kThreads, kCountsAt + static_cast<size_t>(p.width) * 4, 1, stream,
+                             static_cast<const T*>(logits), p);
   }
 };
 
@@ -407,20 +409,8 @@ int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const voi
   }
   if (status != B200_NVFP4_SUCCESS) return status;
   // the second kernel may start while the first one drains: it waits for its end itself
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(num_sequences, l.col_blocks);
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = static_cast<size_t>((num_sequences + 31) / 32) * 4;
-  config.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 1;
-  const cudaError_t launched = cudaLaunchKernelEx(&config, balance_reduce_kernel, p);
-  count_launch();
-  status = launch_status();
-  return launched == cudaSuccess ? status : B200_NVFP4_CUDA_ERROR;
+  return launch_overlapped(balance_reduce_kernel, dim3(num_sequences, l.col_blocks), kThreads, static_cast<size_t>((num_sequences + 31) / 32) * 4, 1,
+                           s, p);
 }
 
 }  // extern "C"

@@ -546,3 +546,53 @@ def test_several_streams_at_once(ops):
     torch.cuda.synchronize()
     for i, outs in enumerate(got):
         assert all(torch.equal(out.view(torch.uint8), want[i]) for out in outs), i
+
+
+def test_launches_that_overlap_keep_their_order(ops):
+    # Kernels may start while their predecessors drain: each reads what the one before wrote, and writes what it
+    # read, over buffers used again at once; with copies and another stream between them; eagerly and captured.
+    m, k, n = 48, 1024, 1024
+    b, sb = weight(n, k, 5)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    inputs = [torch.randn((m, k), device="cuda", generator=g) for _ in range(12)]
+    want = []
+    for x in inputs:
+        y = x
+        for _ in range(2):
+            q, s = ops.quantize_fp8(y)
+            torch.cuda.synchronize()
+            y = ops.fp8_gemm(q, b, s, sb, out_dtype=torch.float32)
+            torch.cuda.synchronize()
+        want.append(y)
+    q, s = torch.empty((m, k), dtype=E4M3, device="cuda"), torch.empty((m, blocks(k)), device="cuda")
+    y, x_in = torch.empty((m, n), device="cuda"), torch.empty((m, k), device="cuda")
+    side = torch.cuda.Stream()
+
+    def chain(x, out, aside):
+        if aside:                                # the input arrives through another stream
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                x_in.copy_(x)
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            x_in.copy_(x)
+        ops.quantize_fp8(x_in, output=q, output_scale=s)
+        ops.fp8_gemm(q, b, s, sb, output=y)
+        ops.quantize_fp8(y, output=q, output_scale=s)
+        ops.fp8_gemm(q, b, s, sb, output=y)
+        out.copy_(y)
+
+    for aside in (False, True):
+        outs = [torch.empty_like(y) for _ in inputs]
+        for _ in range(20):
+            for x, out in zip(inputs, outs):
+                chain(x, out, aside)
+        assert all(torch.equal(a, w) for a, w in zip(outs, want))
+        graph = torch.cuda.CUDAGraph()
+        held = [torch.empty_like(y) for _ in inputs]
+        with torch.cuda.graph(graph):
+            for x, out in zip(inputs, held):
+                chain(x, out, aside)
+        for _ in range(20):
+            graph.replay()
+        assert all(torch.equal(a, w) for a, w in zip(held, want))

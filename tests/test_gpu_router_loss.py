@@ -418,3 +418,41 @@ def test_offsets_beyond_32_bits(ops):
     part = ops.router_backward(z[-ends:].contiguous(), ids[-ends:].contiguous(), topk_weights=w, grad_weights=gw, slope=slope, grad_loss=one,
                                cu_seqlens=near)
     assert torch.equal(grad[-ends:], part)
+
+
+def test_launches_that_overlap_keep_their_order(ops):
+    # loss, its second kernel and the gradient may start while their predecessors drain; ids, sequences and logits
+    # are written right before, over buffers used again at once
+    t, e, k, seqs = 700, 64, 6, 5
+    cases = [case(t, e, k, seqs, i) for i in range(8)]
+    cases = [(z.cuda(), ids.cuda(), cu.cuda(), gw.cuda(), weights_of(z, ids).cuda()) for z, ids, cu, gw in cases]
+    one = torch.ones((), device="cuda")
+
+    def step(z, ids, cu, gw, w, wait):
+        loss, counts, slope = ops.router_balance_loss(z, ids, cu_seqlens=cu)
+        if wait:
+            torch.cuda.synchronize()
+        return loss, counts, slope, ops.router_backward(z, ids, topk_weights=w, grad_weights=gw, slope=slope, grad_loss=one, cu_seqlens=cu)
+
+    want = [step(*c, True) for c in cases]
+    buffers = [torch.empty_like(x) for x in cases[0]]
+
+    def all_cases():
+        got = []
+        for c in cases:
+            for to, x in zip(buffers, c):
+                to.copy_(x)
+            got.append([x.clone() for x in step(*buffers, False)])
+        return got
+
+    for _ in range(10):
+        for a, w in zip(all_cases(), want):
+            assert all(torch.equal(x, y) for x, y in zip(a, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = all_cases()
+    for _ in range(10):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, w in zip(held, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, w))
