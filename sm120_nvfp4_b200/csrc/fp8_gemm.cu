@@ -122,41 +122,75 @@ int launch_pair(const Fp8Problem& q, Fp8Params p, const DeviceInfo& dev, cudaStr
                            tmap_a, tmap_b, tmap_out, p);       // (clusters of two by the kernel's own declaration)
 }
 
-// CTAs per tile over K: as many as still fit the GPU at once and leave each enough blocks of K to pay for the
-// exchange of partial tiles, which grows with the tile (us, tile / splits; 24 x 1024 x 1024: 16/1 6.3,
-// 16/4 5.9; 96 x 1024 x 1024: 64/1 7.6, 64/2 8.7; 64 x 7168 x 2048: 64/1 10.6, 64/2 10.3; 128 x 7168 x 2048: 128/1 12.8, 128/2 14.8;
-// 128 x 4096 x 7168: 128/1 29.5, 128/4 17.2).
-int pick_fp8_splits(const Fp8Problem& q, const DeviceInfo& dev, int tile) {
-  const long long tasks = row_tiles(q, tile) * ((q.n + 127) / 128);
-  const int kb = (q.k + kFp8BlockK - 1) / kFp8BlockK;
-  const int least = tile == 16 ? 2 : (tile == 128 ? 12 : 8);
-  for (int s = 8; s >= 2; s /= 2)
-    if (tasks * s <= dev.sm_count && kb >= least * s) return s;
-  return 1;
+struct Fp8Choice {
+  int tile, splits;      // rows of A per tile (512: 256 x 256 on CTA pairs), CTAs per tile over K
+};
+
+// Microseconds that a launch of `tasks` tiles takes, split over K or not: a fixed part, a part per block of 128 of
+// K that a CTA goes through, a part for the exchange of partial tiles, once more per round of tiles. The
+// constants are fitted to these (rows x N x K, tile / splits: us back to back):
+//   77 x 1000 x 1040    16/1 5.5, 16/2 5.4, 32/1 5.9, 32/4 5.2, 64/1 7.4, 64/4 6.5, 128/1 8.5
+//   77 x 1024 x 4096    16/2 8.3, 32/2 8.9, 32/4 6.6, 64/4 8.1, 128/4 9.8, 128/1 16.9, pairs 18.8
+//   48 x 4096 x 7168    16/1 18.5, 32/2 13.2, 64/2 14.2, 64/4 10.2, 128/2 16.8, 128/4 13.6
+//   128 x 4096 x 7168   32/1 20.0, 64/1 23.2, 64/2 16.0, 128/1 24.6, 128/2 17.4, 128/4 14.0; 192 rows: pairs 29.4
+//   192 x 7168 x 2048   64/1 16.7 (two rounds), 128/1 11.9, pairs 12.6; 384 rows: 128/1 20.1 (two rounds), pairs 13.5
+float fp8_cost(int tile, int splits, long long tasks, int kb, int places) {
+  const float fixed = tile == 16 ? 2.8f : tile == 32 ? 2.9f : tile == 64 ? 3.6f : tile == 128 ? 4.3f : 4.0f;
+  const float per_task = tile == 16 ? 0.5f : tile == 32 ? 0.6f : tile == 64 ? 0.9f : tile == 128 ? 1.2f : 2.0f;
+  const float per_block = tile == 16 ? 0.24f : tile == 32 ? 0.265f : tile == 64 ? 0.33f : tile == 128 ? 0.335f : 0.42f;
+  const float exchange = tile == 16 ? 0.7f : tile == 32 ? 0.9f : tile == 64 ? 1.0f : 2.0f;
+  const long long rounds = (tasks * splits + places - 1) / places;
+  return fixed + static_cast<float>(rounds) * (per_task + per_block * static_cast<float>((kb + splits - 1) / splits)) +
+         (splits > 1 ? exchange : 0.0f);
 }
 
-// Rows of A per tile (512: 256 x 256 on CTA pairs).
-//   Groups: the tile that the average group fills to at most three quarters, since groups differ; every
-//   further tile of a group reads its weights again. 32 groups over 4096 x 7168, us for the average row
-//   counts 12 / 24 / 40 / 64 / 96 / 128: 16 rows 151 / 226 / - , 32 rows 148 / 157 / 218 / 320,
-//   64 rows 164 / 167 / 172 / 256 / 324, 128 rows 177 / 178 / 182 / 185 / 215 / 289, pairs - / - / 216 / 218 /
-//   220 / 219.
-//   One group: the smallest tile that holds all rows up to 64; then 128 rows where K is deep enough to be
-//   split (128 x 4096 x 7168: 17.2 us, 64 rows 17.7) or the tiles fit the GPU at once, 64 rows while even
-//   those do (128 x 7168 x 2048: 11.0 against 12.8), pairs beyond (384 x 7168 x 2048: 14.3 against 22.0).
-int pick_fp8_tile(const Fp8Problem& q, const DeviceInfo& dev) {
-  const int rows = q.avg_rows;
-  if (q.seqlens != nullptr) {
-    for (int tile = 16; tile <= 128; tile *= 2)
-      if (static_cast<long long>(rows) * 4 <= tile * 3) return tile;
-    return kPairTile;
-  }
-  for (int tile = 16; tile <= 64; tile *= 2)
-    if (rows <= tile) return tile;
+// Clusters of 2, 4 and 8 CTAs of the few-row kernel that fit the GPU at once (of 8, fewer than SMs / 8: those of a
+// cluster come from one part of the GPU, and sixteen clusters took 9.1 us where 32 of four took 5.8).
+const int* few_row_clusters(const DeviceInfo& dev) {
+  static std::once_flag once[64];
+  static int fit[64][4];
+  std::call_once(once[dev.device], [&] {
+    auto kernel = fp8_skinny_kernel<16, false>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget) != cudaSuccess) cudaGetLastError();
+    for (int i = 1; i < 4; ++i)
+      fit[dev.device][i] = resident_clusters(kernel, dev, 1 << i, Fp8SkinnyCfg<16, false>::kThreads, kSmemBudget);
+  });
+  return fit[dev.device];
+}
+
+// Tile and splits. One group, or several whose tiles fit the GPU at once: the least estimated time, of all tiles (or
+// `tile` alone) unsplit and of those splits that fit the GPU at once and leave each CTA two blocks.
+// Several groups that do not: the tile that the average group fills to at most three quarters, since groups
+// differ; every further tile of a group reads its weights again. 32 groups over 4096 x 7168, us for the average
+// row counts 12 / 24 / 40 / 64 / 96 / 128: 16 rows 151 / 226 / - , 32 rows 148 / 157 / 218 / 320, 64 rows 164 /
+// 167 / 172 / 256 / 324, 128 rows 177 / 178 / 182 / 185 / 215 / 289, pairs - / - / 216 / 218 / 220 / 219.
+Fp8Choice pick_fp8(const Fp8Problem& q, const DeviceInfo& dev, int tile) {
+  const int kb = (q.k + kFp8BlockK - 1) / kFp8BlockK;
   const long long columns = (q.n + 127) / 128;
-  if (pick_fp8_splits(q, dev, 128) > 1) return 128;
-  if (row_tiles(q, 64) * columns <= dev.sm_count) return 64;
-  return row_tiles(q, 128) * columns <= dev.sm_count ? 128 : kPairTile;
+  const bool grouped = q.seqlens != nullptr;
+  const int* clusters = few_row_clusters(dev);
+  Fp8Choice best{tile == 0 ? kPairTile : tile, 1};
+  float least = 3.4e38f;
+  for (int t = 16; t <= 128; t *= 2) {
+    const long long tasks = row_tiles(q, t) * columns;
+    if ((tile != 0 && tile != t) || (grouped && tasks > dev.sm_count)) continue;
+    for (int i = 0; i == 0 || (i < 4 && tasks <= clusters[i] && kb >= 2 << i); ++i) {
+      const int s = 1 << i;
+      const float cost = fp8_cost(t, s, tasks, kb, dev.sm_count);
+      if (cost < least) {
+        least = cost;
+        best = {t, s};
+      }
+    }
+  }
+  if (tile != 0) return best;
+  if (!grouped) {
+    if (fp8_cost(kPairTile, 1, row_tiles(q, 256) * ((q.n + 255) / 256), kb, dev.sm_count / 2) < least) best = {kPairTile, 1};
+  } else if (least == 3.4e38f) {
+    for (int t = 16; t <= 128; t *= 2)
+      if (static_cast<long long>(q.avg_rows) * 4 <= t * 3) return {t, 1};
+  }
+  return best;
 }
 
 int fp8_product(const Fp8Problem& q, const void* a_scale, const void* b_scale, void* out, int out_type, cudaStream_t stream) {
@@ -179,11 +213,11 @@ int fp8_product(const Fp8Problem& q, const void* a_scale, const void* b_scale, v
   p.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
   p.withhold_first_arrival = g_withhold_once.exchange(0, std::memory_order_relaxed);
   const int forced = g_fp8_tile.load(std::memory_order_relaxed);
-  const int tile = forced ? forced : pick_fp8_tile(q, dev);
-  if (tile == kPairTile) return launch_pair(q, p, dev, stream);
-  int splits = g_fp8_splits.load(std::memory_order_relaxed);
-  if (splits == 0) splits = pick_fp8_splits(q, dev, tile);
-  switch (tile) {
+  const Fp8Choice choice = pick_fp8(q, dev, forced);
+  if (choice.tile == kPairTile) return launch_pair(q, p, dev, stream);
+  const int forced_splits = g_fp8_splits.load(std::memory_order_relaxed);
+  const int splits = forced_splits ? forced_splits : choice.splits;
+  switch (choice.tile) {
     case 16: return launch_skinny<16, false>(q, p, splits, dev, stream);
     case 32: return launch_skinny<32, false>(q, p, splits, dev, stream);
     case 64: return launch_skinny<64, false>(q, p, splits, dev, stream);
