@@ -5,9 +5,9 @@
 //
 // Reads 2 bytes (4 with SiLU) and writes 1.03 per value of a 16-bit input. Eight (or sixteen) lanes share a
 // block: 16-byte loads, an amax by three (four) exchanges, one 16-byte (8-byte) store. 32768 x 4096 BF16:
-// 71 us, 0.87 of what the bytes take at the measured copy rate. 32768 x 2048 with SiLU: 68 us, 0.76 of it: 25
-// instructions per value, half of them the exponential and the division of the SiLU, at 66 % of the issue
-// slots, and the wait for the loads.
+// 69 us, 0.90 of what the bytes take at the measured copy rate. 32768 x 2048 with SiLU: 65.5 us, 0.79 of it: 25
+// instructions per value, half of them the exponential and the division of the SiLU, at 76 % of the issue
+// slots, and the wait for the loads. (Both 2 us more without the overlapped start.)
 //
 // The division: every quotient of a block has the same divisor s, so one correctly rounded reciprocal
 // r = RN(1 / s) serves them all by Markstein's sequence (IBM J. Res. Dev. 34(1), 1990): q0 = RN(x r),

@@ -8,8 +8,9 @@
 // threads that hold the columns add it.
 //
 // Reads the logits, ids, weights and their gradient once and writes the gradient: 8 E + 12 k bytes per
-// token of FP32 logits. 131072 x 160 BF16: 35.6 us where the bytes take 14.2; 65536 x 256 FP32: 31 us (21). Bound by
-// instruction issue (66 to 68 % of the slots), beside the special-function unit's two operations per logit.
+// token of FP32 logits. 131072 x 160 BF16: 30.4 us where the bytes take 14.2; 65536 x 256 FP32: 28.1 us (21). 31
+// instructions per logit at 62 to 64 % of the issue slots, with 16 warps per SM: three blocks per SM
+// instead of two spill (72 us).
 #include "router_common.cuh"
 
 namespace b200 {

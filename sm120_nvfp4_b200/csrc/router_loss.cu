@@ -12,9 +12,11 @@
 // of tokens are written out and added by a second kernel in a fixed order, so that results do not depend
 // on scheduling. Counts are whole numbers and may be added in any order.
 //
-// 65536 x 256 FP32: 27 us where the bytes take 10.6. The first kernel (20 us) is bound by the special-function unit -
-// an exponential and a reciprocal per logit, sixteen a cycle per SM - with half of the issue slots
-// used; the second is 7 us of latencies, of which its early start hides a part. 131072 x 160 BF16: 29 us.
+// 65536 x 256 FP32: 24.8 us where the bytes take 10.6; 131072 x 160 BF16: 25.6 us. In the first kernel no unit is
+// full: the special-function unit is busy for 7.4 us (an exponential and a reciprocal per logit, sixteen a
+// cycle per SM), 44 % of the issue slots are used; with 16 warps per SM the rest is the latency of dependent
+// instructions, and that of the start and the end of blocks with 14 rounds of tokens each. The second
+// kernel is a chain of latencies, 7 us on its own, of which its early start hides a part.
 #include "router_common.cuh"
 
 namespace b200 {
