@@ -168,6 +168,12 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const void* desc,
       : "memory");
 }
 
+// The box of a 2-D tiled load into L2 only, with nothing to wait for.
+__device__ __forceinline__ void tma_prefetch_2d(const void* desc, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(desc)), "r"(c0), "r"(c1)
+               : "memory");
+}
+
 // Same load issued by a CTA of a pair (cta_group::2): the data goes to this CTA's shared
 // memory, the completion bytes to the mbarrier at shared::cluster address `bar_cluster_addr`,
 // which may belong to the other CTA of the pair. Each CTA loads its own tile.
