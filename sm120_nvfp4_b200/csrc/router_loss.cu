@@ -67,12 +67,11 @@ __device__ __forceinline__ int item_sequence(const LossParams& p, int i) {
   return lo;
 }
 
+// Partial sums of one work item, written out. `s_raw`: queues, later a row of sums per group; counts.
 template <typename T, int V, int NV, int G>
-__global__ void __launch_bounds__(kThreads, 2)
-balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
+__device__ __forceinline__ void add_item(const T* __restrict__ logits, const LossParams& p, uint8_t* s_raw, int item) {
   using Gr = Group<G>;
   constexpr int N = V * NV;
-  extern __shared__ __align__(16) uint8_t s_raw[];         // queues, later a row of sums per group; counts
   __shared__ float scratch[kWarps];
   __shared__ int s_live;
   const int lane = Gr::lane();
@@ -82,7 +81,6 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
   rows.fill_rest(p.experts, lane);
   WordQueue<int> first_ids(s_raw + Rows::kBytes);
   int* s_counts = reinterpret_cast<int*>(s_raw + p.counts_at);
-  const int item = blockIdx.x;
   ptx::grid_wait();
   ptx::grid_launch_dependents();                           // the second kernel's blocks may take their places
   if (item == 0 && threadIdx.x == 0) *p.ticket = 0;
@@ -197,31 +195,38 @@ balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
   if (threadIdx.x == 0) p.part_t[item] = make_int2(s, s_live);
 }
 
-// One block per sequence and 64 columns: adds the sequence's partial rows (item order within sixteen
-// interleaved strands, then the strands), and the last block to finish adds up the loss. It is a chain of
-// latencies, so everything that does not depend on the partial sums happens before the first kernel's
-// end is waited for (whatever ran before that kernel has ended: it lets this one start only then), and
-// independent loads are issued together.
-__global__ void __launch_bounds__(kThreads)
-balance_reduce_kernel(const LossParams p) {
-  extern __shared__ unsigned s_filled[];                   // one bit per sequence
-  __shared__ float s_p[16][64];
-  __shared__ int s_n[16][64];
-  __shared__ int s_tokens, s_count;
-  __shared__ double s_loss[kWarps];
-  __shared__ bool s_last;
-  const int s = blockIdx.x, col_block = blockIdx.y;
+template <typename T, int V, int NV, int G>
+__global__ void __launch_bounds__(kThreads, 2)
+balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
+  extern __shared__ __align__(16) uint8_t s_raw[];
+  add_item<T, V, NV, G>(logits, p, s_raw, blockIdx.x);
+}
+
+struct ReduceShared {
+  alignas(16) float p[16][64];             // (written four columns at a time)
+  alignas(16) int n[16][64];
+  int tokens, count;
+  double loss[kWarps];
+};
+static_assert(alignof(ReduceShared) == 16, "rows of four");
+
+// Adds a sequence's partial rows for 64 columns (item order within sixteen interleaved strands, then the strands) and
+// writes counts and slopes; thread 0 gets their part of the loss. It is a chain of latencies, so everything
+// that does not depend on the partial sums happens before `partials_ready` waits for them, and independent
+// loads are issued together. `filled_bits`: one per sequence.
+template <typename Ready>
+__device__ __forceinline__ double reduce_columns(const LossParams& p, int s, int col_block, unsigned* filled_bits, ReduceShared& sh,
+                                                 Ready partials_ready) {
   const int items = p.chunks + p.sequences;
   const int words = (p.sequences + 31) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < words; i += kThreads) s_filled[i] = 0;
-  if (threadIdx.x == 0) { s_tokens = 0; s_count = 0; }
+  for (int i = threadIdx.x; i < words; i += kThreads) filled_bits[i] = 0;
+  if (threadIdx.x == 0) { sh.tokens = 0; sh.count = 0; }
   const int lo = seq_start(p, s), hi = seq_start(p, s + 1);
   const int strand = threadIdx.x >> 4, quad = threadIdx.x & 15;
   const int col = col_block * 64 + quad * 4;
   __syncthreads();
-  ptx::grid_wait();                                        // the partial sums are complete
-  ptx::grid_launch_dependents();
+  partials_ready();
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   int4 num = make_int4(0, 0, 0, 0);
   if (hi > lo && col < p.width) {
@@ -234,20 +239,20 @@ balance_reduce_kernel(const LossParams p) {
       num.x += n.x; num.y += n.y; num.z += n.z; num.w += n.w;
     }
   }
-  *reinterpret_cast<float4*>(&s_p[strand][quad * 4]) = sum;
-  *reinterpret_cast<int4*>(&s_n[strand][quad * 4]) = num;
+  *reinterpret_cast<float4*>(&sh.p[strand][quad * 4]) = sum;
+  *reinterpret_cast<int4*>(&sh.n[strand][quad * 4]) = num;
 #pragma unroll 2
   for (int i = threadIdx.x; i < items; i += kThreads) {
     const int2 t = p.part_t[i];
     if (t.y > 0) {
-      atomicOr(&s_filled[t.x >> 5], 1u << (t.x & 31));
-      if (t.x == s) atomicAdd(&s_tokens, t.y);
+      atomicOr(&filled_bits[t.x >> 5], 1u << (t.x & 31));
+      if (t.x == s) atomicAdd(&sh.tokens, t.y);
     }
   }
   __syncthreads();
   int filled = 0;
-  for (int i = threadIdx.x; i < words; i += kThreads) filled += __popc(s_filled[i]);
-  if (filled) atomicAdd(&s_count, filled);
+  for (int i = threadIdx.x; i < words; i += kThreads) filled += __popc(filled_bits[i]);
+  if (filled) atomicAdd(&sh.count, filled);
   __syncthreads();
   if (threadIdx.x < 64) {
     const int e = col_block * 64 + threadIdx.x;
@@ -255,43 +260,92 @@ balance_reduce_kernel(const LossParams p) {
     int n = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      total += s_p[r][threadIdx.x];
-      n += s_n[r][threadIdx.x];
+      total += sh.p[r][threadIdx.x];
+      n += sh.n[r][threadIdx.x];
     }
     double term = 0.0;
     if (e < p.experts) {
       // alpha E n / (k T^2 S') in FP64, rounded once
-      const double t = s_tokens > 0 ? static_cast<double>(s_tokens) : 1.0;
-      const double slope = static_cast<double>(p.alpha) * p.experts * n / (static_cast<double>(p.topk) * t * t * max(s_count, 1));
+      const double t = sh.tokens > 0 ? static_cast<double>(sh.tokens) : 1.0;
+      const double slope = static_cast<double>(p.alpha) * p.experts * n / (static_cast<double>(p.topk) * t * t * max(sh.count, 1));
       p.counts[static_cast<long long>(s) * p.experts + e] = n;
       p.slope[static_cast<long long>(s) * p.experts + e] = static_cast<float>(slope);
       term = slope * total;
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) term += __shfl_xor_sync(0xffffffffu, term, d);
-    if (lane == 0) s_loss[warp] = term;
+    if (lane == 0) sh.loss[warp] = term;
   }
   __syncthreads();
+  return threadIdx.x == 0 ? sh.loss[0] + sh.loss[1] : 0.0;
+}
+
+// The loss from its parts, by one block, in a fixed order.
+__device__ __forceinline__ void sum_loss(const LossParams& p, long long terms, ReduceShared& sh) {
+  double mine = 0.0;
+  for (long long i = threadIdx.x; i < terms; i += kThreads) mine += __ldcg(p.part_loss + i);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.loss[threadIdx.x >> 5] = mine;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    p.part_loss[static_cast<long long>(s) * gridDim.y + col_block] = s_loss[0] + s_loss[1];
+    double all = 0.0;
+    for (int w = 0; w < kWarps; ++w) all += sh.loss[w];
+    *p.loss = static_cast<float>(all);
+  }
+}
+
+// One block per sequence and 64 columns; the last one to finish adds up the loss. Whatever ran before the first kernel
+// has ended when this one starts: that kernel lets it start only then.
+__global__ void __launch_bounds__(kThreads)
+balance_reduce_kernel(const LossParams p) {
+  extern __shared__ unsigned s_filled[];                   // one bit per sequence
+  __shared__ ReduceShared sh;
+  __shared__ bool s_last;
+  const double part = reduce_columns(p, blockIdx.x, blockIdx.y, s_filled, sh, [] {
+    ptx::grid_wait();                                      // the partial sums are complete
+    ptx::grid_launch_dependents();
+  });
+  if (threadIdx.x == 0) {
+    p.part_loss[static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y] = part;
     __threadfence();
     s_last = atomicAdd(p.ticket, 1u) == gridDim.x * gridDim.y - 1;
   }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  const long long terms = static_cast<long long>(p.sequences) * gridDim.y;
-  double mine = 0.0;
-  for (long long i = threadIdx.x; i < terms; i += kThreads) mine += __ldcg(p.part_loss + i);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0) s_loss[warp] = mine;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0.0;
-    for (int w = 0; w < kWarps; ++w) all += s_loss[w];
-    *p.loss = static_cast<float>(all);
+  sum_loss(p, static_cast<long long>(p.sequences) * gridDim.y, sh);
+}
+
+// Both steps in one launch, for what kOne work items at most hold: a cluster of that many blocks, which meets
+// before the sums are added and before the loss is.
+constexpr int kOne = 8;
+
+template <typename T, int V, int NV, int G>
+__global__ void __cluster_dims__(kOne, 1, 1) __launch_bounds__(kThreads)
+balance_one_kernel(const T* __restrict__ logits, const LossParams p) {
+  extern __shared__ __align__(16) uint8_t s_raw[];
+  __shared__ ReduceShared sh;
+  __shared__ unsigned filled;
+  if (blockIdx.x < p.chunks + p.sequences) {
+    add_item<T, V, NV, G>(logits, p, s_raw, blockIdx.x);
+  } else {
+    ptx::grid_wait();
+    ptx::grid_launch_dependents();
   }
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  const int col_blocks = (p.experts + 63) / 64, parts = p.sequences * col_blocks;
+  for (int i = blockIdx.x; i < parts; i += kOne) {
+    const double part = reduce_columns(p, i / col_blocks, i % col_blocks, &filled, sh, [] {});
+    if (threadIdx.x == 0) p.part_loss[i] = part;
+    __syncthreads();
+  }
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (blockIdx.x == 0) sum_loss(p, parts, sh);
 }
 
 // ---------------------------------------------------------------------------------------- host
@@ -301,21 +355,29 @@ balance_reduce_kernel(const LossParams p) {
 // few items more than that cost a second round: 131072 x 160 BF16 46 us with 467 items on 444 places, 40
 // with 296), with many sequences there are several rounds anyway. Fixed, so that the order of the sums does
 // not depend on the device: 148 SMs.
-int loss_chunk(int tokens, int sequences) {
+int loss_chunk(int tokens, int experts, int sequences) {
   constexpr int kResident = 2 * 148;
   const int chunks = sequences <= kResident / 2 ? kResident - sequences : 2 * kResident;
   const long long chunk = (static_cast<long long>(tokens) + chunks - 1) / chunks;
-  return static_cast<int>(chunk < 32 ? 32 : chunk);
+  const int least = experts <= 512 ? 32 : 4;               // (a block goes through 8 to 32 tokens at a time, or one: 400 x 1024 33 -> 12 us)
+  return static_cast<int>(chunk < least ? least : chunk);
 }
 
 struct LossLayout {
+  bool one;
   int chunk, chunks, width, col_blocks;
   size_t p, n, t, loss, ticket, total;
 };
 
 LossLayout loss_layout(int tokens, int experts, int sequences) {
   LossLayout l;
-  l.chunk = loss_chunk(tokens, sequences);
+  // A call for a few tokens is launches more than anything: where the kOne blocks of a cluster, less one for each
+  // sequence's end, get through the tokens in four steps each, and through the sums in one, one launch does
+  // it all (120 x 64, 3 sequences: 7.6 -> 6.1 us, and 8.7 -> 6.2 on the host; with two rounds of sums
+  // 300 x 160, 3 sequences, took 8.6 against 7.5).
+  const int most = experts <= 256 ? 64 : 32;
+  l.one = sequences < kOne && sequences * ((experts + 63) / 64) <= kOne && tokens <= most * (kOne - sequences);
+  l.chunk = l.one ? (tokens <= 32 * (kOne - sequences) ? 32 : 64) : loss_chunk(tokens, experts, sequences);
   l.chunks = (tokens + l.chunk - 1) / l.chunk;
   l.width = (experts + 3) / 4 * 4;
   l.col_blocks = (experts + 63) / 64;
@@ -332,19 +394,20 @@ LossLayout loss_layout(int tokens, int experts, int sequences) {
 
 template <typename T, int V, int NV, int G>
 struct LossLaunch {
-  static int run(const void* logits, LossParams p, int device, cudaStream_t stream) {
-    static std::once_flag once[64];
-    static cudaError_t status[64];
-    auto kernel = balance_partial_kernel<T, V, NV, G>;
+  static int run(const void* logits, LossParams p, bool one, int device, cudaStream_t stream) {
+    static std::once_flag once[64], once_one[64];
+    static cudaError_t status[64], status_one[64];
+    auto kernel = one ? balance_one_kernel<T, V, NV, G> : balance_partial_kernel<T, V, NV, G>;
     constexpr int kMaxWidth = G > 32 ? kMaxExperts : V * NV * G;
     constexpr size_t kQueues = RowQueue<T, V, NV, G>::kBytes + WordQueue<int>::kBytes;
     constexpr size_t kSums = static_cast<size_t>(Group<G>::kPerBlock) * kMaxWidth * 4;
     constexpr size_t kCountsAt = kQueues > kSums ? kQueues : kSums;
     static_assert(kCountsAt % 16 == 0 && kCountsAt + kMaxWidth * 4 <= 112 * 1024, "two blocks per SM");
-    const int allowed = allow_smem(kernel, once, status, device, static_cast<int>(kCountsAt + kMaxWidth * 4));
+    const int allowed = allow_smem(kernel, one ? once_one : once, one ? status_one : status, device,
+                                   static_cast<int>(kCountsAt + kMaxWidth * 4));
     if (allowed != B200_NVFP4_SUCCESS) return allowed;
     p.counts_at = static_cast<int>(kCountsAt);
-    return launch_overlapped(kernel, p.chunks + p.sequences, kThreads, kCountsAt + static_cast<size_t>(p.width) * 4, 1, stream,
+    return launch_overlapped(kernel, one ? kOne : p.chunks + p.sequences, kThreads, kCountsAt + static_cast<size_t>(p.width) * 4, 1, stream,
                              static_cast<const T*>(logits), p);
   }
 };
@@ -405,11 +468,11 @@ int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const voi
   const bool quads = num_experts % 4 == 0 && aligned(logits, 4 * size);
   int status;
   switch (logits_dtype) {
-    case 0: status = dispatch_width<__half, LossLaunch>(num_experts, quads, logits, p, dev.device, s); break;
-    case 1: status = dispatch_width<__nv_bfloat16, LossLaunch>(num_experts, quads, logits, p, dev.device, s); break;
-    default: status = dispatch_width<float, LossLaunch>(num_experts, quads, logits, p, dev.device, s); break;
+    case 0: status = dispatch_width<__half, LossLaunch>(num_experts, quads, logits, p, l.one, dev.device, s); break;
+    case 1: status = dispatch_width<__nv_bfloat16, LossLaunch>(num_experts, quads, logits, p, l.one, dev.device, s); break;
+    default: status = dispatch_width<float, LossLaunch>(num_experts, quads, logits, p, l.one, dev.device, s); break;
   }
-  if (status != B200_NVFP4_SUCCESS) return status;
+  if (status != B200_NVFP4_SUCCESS || l.one) return status;
   // the second kernel may start while the first one drains: it waits for its end itself
   return launch_overlapped(balance_reduce_kernel, dim3(num_sequences, l.col_blocks), kThreads, static_cast<size_t>((num_sequences + 31) / 32) * 4, 1,
                            s, p);

@@ -420,10 +420,11 @@ def test_offsets_beyond_32_bits(ops):
     assert torch.equal(grad[-ends:], part)
 
 
-def test_launches_that_overlap_keep_their_order(ops):
-    # loss, its second kernel and the gradient may start while their predecessors drain; ids, sequences and logits
+@pytest.mark.parametrize("t,seqs", [(700, 5), (150, 3)])
+def test_launches_that_overlap_keep_their_order(ops, t, seqs):
+    # loss, its second kernel (the smaller case has none) and the gradient may start while their predecessors drain; ids, sequences and logits
     # are written right before, over buffers used again at once
-    t, e, k, seqs = 700, 64, 6, 5
+    e, k = 64, 6
     cases = [case(t, e, k, seqs, i) for i in range(8)]
     cases = [(z.cuda(), ids.cuda(), cu.cuda(), gw.cuda(), weights_of(z, ids).cuda()) for z, ids, cu, gw in cases]
     one = torch.ones((), device="cuda")
@@ -456,3 +457,17 @@ def test_launches_that_overlap_keep_their_order(ops):
     torch.cuda.synchronize()
     for a, w in zip(held, want):
         assert all(torch.equal(x, y) for x, y in zip(a, w))
+
+
+@pytest.mark.parametrize("t,e,k,seqs", [(64 * 7, 64, 4, 1), (64 * 7 + 1, 64, 4, 1), (32 * 4 + 1, 128, 8, 4), (64, 60, 3, 7), (65, 60, 3, 7),
+                                        (30, 64, 2, 8), (224, 512, 8, 1), (225, 512, 8, 1), (9, 5, 2, 6), (448, 600, 4, 2)])
+def test_around_what_one_launch_takes(ops, t, e, k, seqs):
+    z, ids, cu, gw = case(t, e, k, seqs, t + e + seqs)
+    loss, counts, slope = ops.router_balance_loss(z.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
+    wl, wc, ws, live, seq = reference(z, ids, cu, "sigmoid", 1.0)
+    assert torch.equal(counts.cpu().long(), wc)
+    assert ((slope.cpu().double() - ws).abs() <= ws * 2.0 ** -23).all()
+    # a sum of positive terms: the score's error, and at most 64 additions of a block's rows and 16 + 8 of partial rows
+    assert abs(float(loss) - float(wl)) <= float(wl) * (float(score_error(z).max()) * 2 + 96 * 2.0 ** -24)
+    again = ops.router_balance_loss(z.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
+    assert all(torch.equal(a, b) for a, b in zip((loss, counts, slope), again))
