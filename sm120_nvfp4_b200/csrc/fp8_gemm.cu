@@ -60,6 +60,13 @@ long long row_tiles(const Fp8Problem& q, int tile_rows) {
   return q.seqlens == nullptr ? exact : static_cast<long long>(q.rows) / tile_rows + (q.rows < q.groups ? q.rows : q.groups);
 }
 
+// The same, but what is likely for several: every group ends in a tile that is half empty on average.
+long long likely_row_tiles(const Fp8Problem& q, int tile_rows) {
+  if (q.seqlens == nullptr) return row_tiles(q, tile_rows);
+  const long long tiles = static_cast<long long>(q.rows) / tile_rows + (q.groups + 1) / 2, least = q.rows < q.groups ? q.rows : q.groups;
+  return tiles > least ? tiles : least;
+}
+
 template <int BN, bool kWide>
 int launch_skinny(const Fp8Problem& q, Fp8Params p, int splits, const DeviceInfo& dev, cudaStream_t stream) {
   using Cfg = Fp8SkinnyCfg<BN, kWide>;
@@ -158,8 +165,9 @@ const int* few_row_clusters(const DeviceInfo& dev) {
   return fit[dev.device];
 }
 
-// Tile and splits. One group, or several whose tiles fit the GPU at once: the least estimated time, of all tiles (or
-// `tile` alone) unsplit and of those splits that fit the GPU at once and leave each CTA two blocks.
+// Tile and splits. One group, or several whose tiles are likely to fit the GPU at once (16 groups, 100 rows, 1024 x
+// 2048: 16/1 8.3, 64/1 10.6; 4 groups, 64 rows, 4096 x 2048: 32/1 8.7, 64/1 10.3): the least estimated time, of all
+// tiles (or `tile` alone) unsplit and of those splits that certainly fit at once and leave each CTA two blocks.
 // Several groups that do not: the tile that the average group fills to at most three quarters, since groups
 // differ; every further tile of a group reads its weights again. 32 groups over 4096 x 7168, us for the average
 // row counts 12 / 24 / 40 / 64 / 96 / 128: 16 rows 151 / 226 / - , 32 rows 148 / 157 / 218 / 320, 64 rows 164 /
@@ -172,9 +180,9 @@ Fp8Choice pick_fp8(const Fp8Problem& q, const DeviceInfo& dev, int tile) {
   Fp8Choice best{tile == 0 ? kPairTile : tile, 1};
   float least = 3.4e38f;
   for (int t = 16; t <= 128; t *= 2) {
-    const long long tasks = row_tiles(q, t) * columns;
+    const long long tasks = likely_row_tiles(q, t) * columns, most = row_tiles(q, t) * columns;
     if ((tile != 0 && tile != t) || (grouped && tasks > dev.sm_count)) continue;
-    for (int i = 0; i == 0 || (i < 4 && tasks <= clusters[i] && kb >= 2 << i); ++i) {
+    for (int i = 0; i == 0 || (i < 4 && most <= clusters[i] && kb >= 2 << i); ++i) {
       const int s = 1 << i;
       const float cost = fp8_cost(t, s, tasks, kb, dev.sm_count);
       if (cost < least) {
