@@ -33,7 +33,13 @@
 //
 // Both start while the kernel before them drains: barriers, tensor memory and descriptors are set up by the time
 // that one has ended (one row, 4096 x 7168: 12.3 -> 9.0 us back to back, 4096 x 4096 x 7168 136 -> 129).
-// All waits are bounded (ptx::mbar_wait) and reported through the device error word.
+//
+// Waits on barriers in shared memory are bounded (ptx::mbar_wait_warp: one answer per warp) and reported through the
+// device error word. Three others have no limit. The barriers of a cluster: its CTAs run at the same time, and all
+// arrive, after a wait that has run out too. griddepcontrol.wait: it ends with the kernel before. The allocation
+// of tensor memory, which comes before griddepcontrol.wait: a block of these kernels takes more than 200 of an SM's 228
+// KB of shared memory, so no other of them and no four-bit product, which all use more than the rest, can be there
+// with tensor memory of its own while this one waits for theirs.
 #pragma once
 
 #include <type_traits>
@@ -175,6 +181,7 @@ struct Fp8SkinnyCfg {
     return fixed_bytes(groups, splits) + stages_for(groups, splits) * kStageBytes;
   }
   static_assert(stages_for(kMaxGroups, 2) >= 4 && stages_for(kMaxGroups, 2) * kStageBytes >= kRedBytes, "ring too small");
+  static_assert(smem_bytes(1, 1) > 200 * 1024 && smem_bytes(1, 2) > 200 * 1024, "one block per SM: see the allocation of tensor memory");
 };
 
 template <int BN, bool kWide>
@@ -263,6 +270,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   } else {
     fp8_group_tables(p, Cfg::kTileM, s_cu_tiles, s_row0, s_rows);
   }
+  __syncwarp();
   if (splits > 1) ptx::cluster_arrive_relaxed();
   ptx::tc_fence_after_sync();
 
@@ -274,7 +282,9 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   const int task_step = splits > 1 ? total_tasks : static_cast<int>(gridDim.x);
   const uint32_t stage_u32 = ptx::smem_u32(smem);
   // Threads of a cluster wait for each other twice: `met`, this warp has waited for the set-up of the others'
-  // barriers; `done`, it has said that it needs nothing of the others any more.
+  // barriers; `done`, it has said that it needs nothing of the others any more. Both are the same in all lanes
+  // of a warp, on the way out of a wait that has run out too: a lane that took its own way would be counted
+  // in the wrong phase.
   bool met = false, done = false;
   // (a single row of tiles needs none of the divisions: they stood 0.6 us before the first load)
   auto decode = [&](int task) {
@@ -293,7 +303,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       const TileCoord t = decode(task);
       const int row = rows_of_a ? s_row0[t.g] + t.mt * Cfg::kTileM : t.g * p.n + t.nt * Cfg::kTileN;
       for (int b = b_begin; b < b_end; ++b) {
-        if (!ptx::mbar_wait(empty_u32 + 8 * stage, phase ^ 1, abort_flag, kWaitEmpty, p.wait_limit)) { ok = false; break; }
+        if (!ptx::mbar_wait_warp(empty_u32 + 8 * stage, phase ^ 1, abort_flag, kWaitEmpty, p.wait_limit)) { ok = false; break; }
         if (ptx::elect_one()) {
           const uint32_t bar = full_u32 + 8 * stage;
           if (withhold) withhold = false;
@@ -313,8 +323,8 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     bool ok = true;
     for (int task = first_task; task < total_tasks && ok; task += task_step) {
       for (int b = b_begin; b < b_end; ++b) {
-        if (!ptx::mbar_wait(sum_empty_u32 + 8 * buf, buf_phase ^ 1, abort_flag, kWaitAccEmpty, p.wait_limit) ||
-            !ptx::mbar_wait(full_u32 + 8 * stage, phase, abort_flag, kWaitFull, p.wait_limit)) { ok = false; break; }
+        if (!ptx::mbar_wait_warp(sum_empty_u32 + 8 * buf, buf_phase ^ 1, abort_flag, kWaitAccEmpty, p.wait_limit) ||
+            !ptx::mbar_wait_warp(full_u32 + 8 * stage, phase, abort_flag, kWaitFull, p.wait_limit)) { ok = false; break; }
         ptx::tc_fence_after_sync();
         if (ptx::elect_one()) {
           const uint32_t wide_lo = lo0 + stage * (Cfg::kStageBytes >> 4);
@@ -383,13 +393,13 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         if (lane == 0) ptx::mbar_arrive(sc_full_u32 + 8 * panel);
         if (b + kFp8Panel < b_end) fetch_scales(task, b + kFp8Panel);
         else if (task + task_step < total_tasks) fetch_scales(task + task_step, b_begin);
-        if (!ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) return false;
+        if (!ptx::mbar_wait_warp(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) return false;
         sc = to;
         if (++panel == kFp8Panels) { panel = 0; panel_phase ^= 1; }
         return true;
       };
       auto sums_ready = [&] {
-        if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) return false;
+        if (!ptx::mbar_wait_warp(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) return false;
         ptx::tc_fence_after_sync();
         return true;
       };
@@ -490,9 +500,10 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(part_full_u32);
+        __syncwarp();                                              // (the barriers of a cluster are for whole warps)
         ptx::cluster_wait();                                       // every CTA has its barriers
         met = true;
-        if (!ptx::mbar_wait(part_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
+        if (!ptx::mbar_wait_warp(part_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
         const uint32_t red_u32 = ptx::smem_u32(red);
         if (first) {
           for (int d = 0; d < splits; ++d) {
@@ -503,7 +514,8 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                                   ptx::map_to_cta(red_full_u32, d));
           }
         }
-        if (mine > 0 && !ptx::mbar_wait_cluster(red_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
+        if (mine > 0 && !ptx::mbar_wait_cluster_warp(red_full_u32, 0, abort_flag, kWaitPartials, p.wait_limit)) break;
+        __syncwarp();
         ptx::cluster_arrive_relaxed();       // the others' copies have landed here (the wait is in the teardown)
         done = true;
         if (mine > 0) {
@@ -628,6 +640,7 @@ struct Fp8PairCfg {
   static constexpr int smem_bytes(int groups) { return fixed_bytes(groups) + stages_for(groups) * kStageBytes; }
 };
 static_assert(Fp8PairCfg::stages_for(kMaxGroups) >= 4, "pipeline too shallow");
+static_assert(Fp8PairCfg::smem_bytes(1) > 200 * 1024, "one block per SM: see the allocation of tensor memory");
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -716,7 +729,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const TileCoord t = decode_tile(task, total_mt, n_tiles, 1, p.raster_m, s_cu_tiles, p.num_groups);
       const int row = is_a ? s_row0[t.g] + t.mt * 256 + cta * 128 : t.g * p.n + t.nt * 256 + cta * 128;
       for (int b = 0; b < kb; ++b) {
-        if (!ptx::mbar_wait(empty_u32 + 8 * stage, phase ^ 1, abort_flag, kWaitEmpty, p.wait_limit)) { ok = false; break; }
+        if (!ptx::mbar_wait_warp(empty_u32 + 8 * stage, phase ^ 1, abort_flag, kWaitEmpty, p.wait_limit)) { ok = false; break; }
         if (ptx::elect_one()) {
           if (withhold) withhold = false;
           else if (leader) ptx::mbar_arrive_expect_tx(full_u32 + 8 * stage, 2 * Cfg::kABytes);   // both CTAs' halves
@@ -738,7 +751,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const int valid = min(128, s_rows[t.g] - t.mt * 256 - cta * 128);     // may be <= 0 in the second CTA
       const float* sb = p.b_scale + (static_cast<long long>(t.g) * nb + 2 * t.nt) * kb;
       for (int b0 = 0; b0 < kb; b0 += Cfg::kPanel) {
-        if (!ptx::mbar_wait(sc_empty_u32 + 8 * panel, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
+        if (!ptx::mbar_wait_warp(sc_empty_u32 + 8 * panel, phase ^ 1, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
         const uint32_t dst = ptx::smem_u32(slots + panel * Cfg::kPanelFloats);
         if (p.scales_by_16) {
 #pragma unroll
@@ -775,8 +788,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       bool ok = true;
       for (int task = first_task; task < total_tasks && ok; task += task_step) {
         for (int b = 0; b < kb; ++b) {
-          if (!ptx::mbar_wait(full_u32 + 8 * stage, phase, abort_flag, kWaitFull, p.wait_limit) ||
-              !ptx::mbar_wait(sum_empty_u32 + 8 * buf, buf_phase ^ 1, abort_flag, kWaitAccEmpty, p.wait_limit)) { ok = false; break; }
+          if (!ptx::mbar_wait_warp(full_u32 + 8 * stage, phase, abort_flag, kWaitFull, p.wait_limit) ||
+              !ptx::mbar_wait_warp(sum_empty_u32 + 8 * buf, buf_phase ^ 1, abort_flag, kWaitAccEmpty, p.wait_limit)) { ok = false; break; }
           ptx::tc_fence_after_sync();
           if (ptx::elect_one()) {
             const uint32_t a_lo = lo0 + stage * (Cfg::kStageBytes >> 4);
@@ -815,7 +828,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       float4 s4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int b = 0; b < kb; ++b) {
         if ((b & (Cfg::kPanel - 1)) == 0) {
-          if (!ptx::mbar_wait(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
+          if (!ptx::mbar_wait_warp(sc_full_u32 + 8 * panel, panel_phase, abort_flag, kWaitSlots, p.wait_limit)) { ok = false; break; }
           const float4* sc = reinterpret_cast<const float4*>(slots + panel * Cfg::kPanelFloats);
           const float4 sa = sc[q * 32 + lane], sb = sc[128 + half];
           s4 = make_float4(sa.x * sb.x, sa.y * sb.y, sa.z * sb.z, sa.w * sb.w);
@@ -825,7 +838,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
         const float s = s4.x;
         s4 = make_float4(s4.y, s4.z, s4.w, s4.x);
-        if (!ptx::mbar_wait(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
+        if (!ptx::mbar_wait_warp(sum_full_u32 + 8 * buf, buf_phase, abort_flag, kWaitAccFull, p.wait_limit)) { ok = false; break; }
         ptx::tc_fence_after_sync();
         const uint32_t from = addr + buf * 256;
 #pragma unroll

@@ -152,6 +152,28 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
   }
 }
 
+// The same waits by a whole warp, with one answer for all its lanes. Lanes that ran out of time on their own
+// would come apart from the others in front of instructions that a warp executes as one (elections, aligned
+// barriers, loads from tensor memory), and count a cluster's barrier wrongly.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code,
+                                               long long limit) {
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+  const long long start = clock64();
+  uint32_t spins = 0;
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((++spins & 255u) == 0) {
+      const bool late = clock64() - start > limit;
+      if (late) atomicCAS(const_cast<int*>(abort_flag), 0, code);
+      if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait_cluster_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code,
+                                                       long long limit) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, abort_flag, code, limit)) != 0;
+}
+
 // --------------------------------------------------------------------- TMA
 
 __device__ __forceinline__ void prefetch_tensormap(const void* desc) {

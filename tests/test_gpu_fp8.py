@@ -618,3 +618,29 @@ def test_weights_written_by_the_kernel_before(ops):
             got.append(ops.fp8_gemm(a, b, sa, sb))
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % 4]), i
+
+
+@pytest.mark.parametrize("tile,splits,m", [(16, 8, 9), (32, 2, 30), (64, 2, 40), (64, 8, 40), (128, 1, 100), (128, 2, 100), (128, 4, 100)])
+def test_clusters_leave_together_when_a_wait_runs_out(ops, L, tile, splits, m):
+    # The warps of a cluster whose waits run out still meet its barriers, each warp as one: the launch ends, reports the wait,
+    # and the next ones are right; for one group and for several.
+    from sm120_nvfp4_b200 import _lib
+    n, k = 264, 2048
+    a, sa = codes(m, k, 1)
+    pairs = [weight(n, k, i) for i in (2, 5)]
+    b, sb = pairs[0]
+    w, sw = torch.stack([p[0].view(torch.uint8) for p in pairs]).view(E4M3), torch.stack([p[1] for p in pairs])
+    n1 = torch.tensor([m // 2, m - m // 2], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda")
+    assert L.b200_nvfp4_fp8_set_tile(tile, splits) == 0
+    calls = [lambda: ops.fp8_gemm(a, b, sa, sb), lambda: ops.fp8_grouped_gemm(a, w, n1, cu, sa, sw)]
+    for call in calls:
+        want = call()
+        for _ in range(2):
+            try:
+                assert L.b200_nvfp4_set_wait_limit(20_000_000, 1) == 0
+                call()
+                assert _lib.device_error() & 0xff in range(1, 9)
+            finally:
+                L.b200_nvfp4_set_wait_limit(0, 0)
+            assert torch.equal(call(), want) and _lib.device_error() == 0
