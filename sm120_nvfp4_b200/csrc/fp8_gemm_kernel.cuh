@@ -359,11 +359,11 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       const int j = tid & 7;
       const float* src = p.a_scale + static_cast<long long>(s_row0[t.g] + t.mt * Cfg::kTileM) * kb + b0 + j;
       const long long tile = static_cast<long long>(t.g) * ((p.n + 127) / 128) + t.nt * Cfg::kTileN / 128;
-      next_w_scale = b0 + j < b_end ? __ldg(p.b_scale + tile * kb + b0 + j) : 0.0f;
+      next_w_scale = b0 + j < b_end ? p.b_scale[tile * kb + b0 + j] : 0.0f;
 #pragma unroll
       for (int i = 0; i < Cfg::kScales; ++i) {
         const int r = (tid >> 3) + i * (4 * Cfg::kPromoters);
-        next_scale[i] = r < left && b0 + j < b_end ? __ldg(src + static_cast<long long>(r) * kb) : 0.0f;
+        next_scale[i] = r < left && b0 + j < b_end ? src[static_cast<long long>(r) * kb] : 0.0f;
       }
     };
     int buf = 0, panel = 0;

@@ -151,7 +151,7 @@ __device__ __forceinline__ void silu_mul(float (&v)[N], const float (&u)[N]) {
 // thread's kUnroll blocks is, in rows and blocks (the blocks a thread block handles at a time / kb, % kb).
 template <typename T, bool kSwiglu, int kPer, int kUnroll>
 __global__ void __launch_bounds__(256, kPer == 16 ? 5 : 0)
-fp8_quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const T* __restrict__ x, int k, uint32_t kb,
+fp8_quantize_kernel(uint8_t* q, float* scale, const T* x, int k, uint32_t kb,
                     uint32_t blocks, uint32_t step_rows, uint32_t step_cols) {
   constexpr int kLanes = 128 / kPer;
   constexpr uint32_t kAtOnce = 256 / kLanes;

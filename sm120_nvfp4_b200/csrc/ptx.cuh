@@ -473,7 +473,10 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 
 // A kernel launched with programmatic stream serialization may start while the one before it in its stream
 // drains. grid_wait() returns once that one has finished and its writes can be seen: every thread calls
-// it before it touches global memory, and before any wait whose time is limited.
+// it before it touches global memory, and before any wait whose time is limited. What such a kernel reads
+// through plain pointers may still be written when it starts, so none of them is `const __restrict__` or read by __ldg:
+// either would promise the compiler that nobody writes there while the kernel lives, and let it use the read-only path or
+// move the load up over the wait.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // The next kernel of the stream may be started where places are free (it waits for this one's end itself).
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }

@@ -32,7 +32,7 @@ struct GradParams {
 
 template <typename T, int V, int NV, int G>
 __global__ void __launch_bounds__(kThreads, 2)
-router_grad_kernel(T* __restrict__ grad, const T* __restrict__ logits, const GradParams p) {
+router_grad_kernel(T* grad, const T* logits, const GradParams p) {
   using Gr = Group<G>;
   constexpr int N = V * NV;
   extern __shared__ __align__(16) uint8_t s_raw[];         // queues; per group the weights' part of a row, and owners

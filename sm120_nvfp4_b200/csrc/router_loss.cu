@@ -69,7 +69,7 @@ __device__ __forceinline__ int item_sequence(const LossParams& p, int i) {
 
 // Partial sums of one work item, written out. `s_raw`: queues, later a row of sums per group; counts.
 template <typename T, int V, int NV, int G>
-__device__ __forceinline__ void add_item(const T* __restrict__ logits, const LossParams& p, uint8_t* s_raw, int item) {
+__device__ __forceinline__ void add_item(const T* logits, const LossParams& p, uint8_t* s_raw, int item) {
   using Gr = Group<G>;
   constexpr int N = V * NV;
   __shared__ float scratch[kWarps];
@@ -197,7 +197,7 @@ __device__ __forceinline__ void add_item(const T* __restrict__ logits, const Los
 
 template <typename T, int V, int NV, int G>
 __global__ void __launch_bounds__(kThreads, 2)
-balance_partial_kernel(const T* __restrict__ logits, const LossParams p) {
+balance_partial_kernel(const T* logits, const LossParams p) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   add_item<T, V, NV, G>(logits, p, s_raw, blockIdx.x);
 }
@@ -324,7 +324,7 @@ constexpr int kOne = 8;
 
 template <typename T, int V, int NV, int G>
 __global__ void __cluster_dims__(kOne, 1, 1) __launch_bounds__(kThreads)
-balance_one_kernel(const T* __restrict__ logits, const LossParams p) {
+balance_one_kernel(const T* logits, const LossParams p) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   __shared__ ReduceShared sh;
   __shared__ unsigned filled;

@@ -177,3 +177,16 @@ def test_python_surface_refuses_wrong_shapes_and_types():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_kernels_that_start_early_make_no_read_only_loads():
+    # they run beside the kernel that still writes what they read, so nothing of it may be declared unchanging
+    import re
+    from pathlib import Path
+    import sm120_nvfp4_b200
+    sources = [p for p in sorted((Path(sm120_nvfp4_b200.__file__).parent / "csrc").glob("*.cu*")) if p.name != "ptx.cuh"]
+    early = [p for p in sources if "grid_wait()" in p.read_text()]
+    assert {"fp8_gemm_kernel.cuh", "fp8_quant.cu", "router_loss.cu", "router_grad.cu"} <= {p.name for p in early}
+    for p in early + [p for p in sources if p.name == "router_common.cuh"]:
+        code = re.sub(r"//[^\n]*", "", p.read_text())
+        assert not re.search(r"__ldg|__restrict__|\.nc\b", code), p.name

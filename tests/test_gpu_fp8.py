@@ -644,3 +644,53 @@ def test_clusters_leave_together_when_a_wait_runs_out(ops, L, tile, splits, m):
             finally:
                 L.b200_nvfp4_set_wait_limit(0, 0)
             assert torch.equal(call(), want) and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [24, 700])
+def test_expert_layers_that_overlap_keep_their_order(ops, rows, dtype):
+    # quantiser, gate/up products, quantiser with SiLU, down products: each starts while the one before still writes what it
+    # reads, over buffers used again at once; eagerly and captured
+    e, h, inter = 6, 512, 384
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    inputs = [torch.randn((rows, h), device="cuda", generator=g).to(dtype) for _ in range(8)]
+    n1 = torch.full((e,), rows // e, dtype=torch.int32, device="cuda")
+    cu = torch.arange(e + 1, dtype=torch.int32, device="cuda") * (rows // e)
+    stack = lambda n, k, at: [torch.stack(x) for x in zip(*((a.view(torch.uint8), b) for a, b in (weight(n, k, at + i) for i in range(e))))]  # noqa: E731
+    (gw, gs), (dw, ds) = stack(2 * inter, h, 10), stack(h, inter, 30)
+    x_in, mid, out = (torch.empty((rows, c), dtype=dtype, device="cuda") for c in (h, 2 * inter, h))
+    q1, s1 = torch.empty((rows, h), dtype=E4M3, device="cuda"), torch.empty((rows, blocks(h)), device="cuda")
+    q2, s2 = torch.empty((rows, inter), dtype=E4M3, device="cuda"), torch.empty((rows, blocks(inter)), device="cuda")
+    mid.zero_(), out.zero_()
+
+    def layer(x, to, wait):
+        meet = torch.cuda.synchronize if wait else lambda: None
+        x_in.copy_(x)
+        for _ in range(2):                       # (the second layer reads the first one's output)
+            ops.quantize_fp8(x_in, output=q1, output_scale=s1)
+            meet()
+            ops.fp8_grouped_gemm(q1, gw, n1, cu, s1, gs, output=mid)
+            meet()
+            ops.quantize_fp8(mid, swiglu=True, output=q2, output_scale=s2)
+            meet()
+            ops.fp8_grouped_gemm(q2, dw, n1, cu, s2, ds, output=out)
+            meet()
+            x_in.copy_(out)
+        to.copy_(out)
+
+    want, got, held = ([torch.empty_like(out) for _ in inputs] for _ in range(3))
+    for x, to in zip(inputs, want):
+        layer(x, to, True)
+    for _ in range(20):
+        for x, to in zip(inputs, got):
+            layer(x, to, False)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for x, to in zip(inputs, held):
+            layer(x, to, False)
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    bits = lambda xs: [x.view(torch.int16) for x in xs]  # noqa: E731
+    for a, b, c in zip(bits(got), bits(held), bits(want)):
+        assert torch.equal(a, c) and torch.equal(b, c)
