@@ -122,8 +122,10 @@ __device__ __forceinline__ void minus_quotients(float (&v)[N], float s, float y)
 }
 
 // silu(g) * u = g / (1 + e^-g) * u. The quotient is Markstein's sequence again, here on the reciprocal
-// instruction, which is one unit off at most: the corrected quotient is off by half a unit and 2^-21 of one
-// at most, so it is the IEEE division's but for one value in some 2^20 (none in 2^27 random ones; 80 -> 72 us). It is computed with its sign turned
+// instruction, which is one unit off at most: its proof leaves the correction 2^-21 of a unit of the quotient off, enough
+// to round the other way next to a midpoint. No gate is there: over all 2237399042 FP32 values of g in [-87, 87] the
+// result is the IEEE division's to the bit (on B200), so a value does not depend on which of the two ways its
+// thread takes. (With the rounded reciprocal 80 us instead of 72.) It is computed with its sign turned
 // round for the sake of zeros, as above, and -u turns it back. Gates beyond 87, whose divisor or remainder could
 // leave the range, send the thread's values through IEEE divisions (the divisor is below 2^126 otherwise).
 template <int N>

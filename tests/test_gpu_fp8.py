@@ -694,3 +694,30 @@ def test_expert_layers_that_overlap_keep_their_order(ops, rows, dtype):
     bits = lambda xs: [x.view(torch.int16) for x in xs]  # noqa: E731
     for a, b, c in zip(bits(got), bits(held), bits(want)):
         assert torch.equal(a, c) and torch.equal(b, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_silu_does_not_depend_on_the_values_beside_it(ops, dtype):
+    """Every 16-bit gate, and FP32 ones of every exponent, one per block: its scale, which shows the bits of silu(gate) * up, is
+    the same with a gate of 100 in the same thread (whose values then take plain divisions) and in a batch of another size."""
+    if dtype == torch.float32:
+        bits = torch.randint(-2 ** 31, 2 ** 31, (1 << 18,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+        gates = bits.view(torch.float32)
+    else:
+        gates = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(dtype)
+    gates = gates[gates.float().abs() <= 87.0]
+    for up in (1.0, -1.375):
+        x = torch.zeros((gates.numel(), 256), dtype=dtype, device="cuda")
+        x[:, 0], x[:, 128] = gates.cuda(), up
+        q, s = ops.quantize_fp8(x, swiglu=True)
+        parts = [ops.quantize_fp8(x[i:i + 200].contiguous(), swiglu=True) for i in range(0, min(20000, x.shape[0]), 200)]
+        few = sum(p[1].shape[0] for p in parts)
+        assert torch.equal(s[:few], torch.cat([p[1] for p in parts]))
+        assert torch.equal(q[:few].view(torch.uint8), torch.cat([p[0].view(torch.uint8) for p in parts]))
+        x[:, 1] = 100.0                                # times an up of zero
+        q2, s2 = ops.quantize_fp8(x, swiglu=True)
+        assert torch.equal(s, s2) and torch.equal(q.view(torch.uint8), q2.view(torch.uint8))
+        # and it is the rounded value: exp 2 units, sum, quotient, product and scale half a unit each
+        v = gates.double() / (1.0 + torch.exp(-gates.double())) * up
+        want = v.abs().clamp(min=2.0 ** -60) / 448.0
+        assert ((s[:, 0].cpu().double() - want).abs() <= 8 * 2.0 ** -24 * want).all()
