@@ -12,6 +12,11 @@
 // of tokens are written out and added by a second kernel in a fixed order, so that results do not depend
 // on scheduling. Counts are whole numbers and may be added in any order.
 //
+// Probabilities are added in FP32 for kRun tokens at most, then in FP64: equal ones (an indifferent router's) are
+// rounded the same way again and again, and one FP32 sum over n of them is off by up to n 2^-25 (2^22 tokens x 520: 1.7e-4,
+// 2^26 x 7: 8e-5; now below 3e-7 both). A run is off by 2^-21 at most, whatever the number of tokens. It costs nothing at
+// 65536 x 256, 0.5 us at 4096 x 256 (8.5) and 3 % beyond 512 experts.
+//
 // 65536 x 256 FP32: 24.8 us where the bytes take 10.6; 131072 x 160 BF16: 25.6 us. In the first kernel no unit is
 // full: the special-function unit is busy for 7.4 us (an exponential and a reciprocal per logit, sixteen a
 // cycle per SM), 44 % of the issue slots are used; with 16 warps per SM the rest is the latency of dependent
@@ -28,11 +33,11 @@ struct LossParams {
   const int* cu;              // [S + 1] or nullptr: one sequence of all tokens
   int tokens, experts, topk, sequences;
   int chunk, chunks;          // tokens per chunk, number of chunks
-  int width;                  // experts rounded up to 4: floats per partial row
+  int width;                  // experts rounded up to 4: values per partial row
   int counts_at;              // place of the counts in shared memory
   float alpha;
   int softmax;
-  float* part_p;              // [chunks + sequences, width]
+  double* part_p;             // [chunks + sequences, width]
   int* part_n;                // same
   int2* part_t;               // [chunks + sequences] (sequence, live tokens)
   double* part_loss;          // [sequences, column blocks]
@@ -67,7 +72,20 @@ __device__ __forceinline__ int item_sequence(const LossParams& p, int i) {
   return lo;
 }
 
-// Partial sums of one work item, written out. `s_raw`: queues, later a row of sums per group; counts.
+// value(0) + ... + value(N - 1), as four sums side by side: additions in FP64 that wait for each other take long.
+template <int N, typename Value>
+__device__ __forceinline__ double sum_rows(Value value) {
+  static_assert(N % 4 == 0, "four sums");
+  double s[4] = {value(0), value(1), value(2), value(3)};
+#pragma unroll
+  for (int r = 4; r < N; ++r) s[r & 3] += value(r);
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+constexpr int kRun = 16;       // additions in FP32 before a sum goes into its FP64 one
+
+// Partial sums of one work item, written out. `s_raw`: queues, a row of sums per group, counts. (The one group of a
+// wide row adds up in its partial row itself: 32 KB of sums per block would leave room for one block per SM only.)
 template <typename T, int V, int NV, int G>
 __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, uint8_t* s_raw, int item) {
   using Gr = Group<G>;
@@ -75,11 +93,11 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
   __shared__ float scratch[kWarps];
   __shared__ int s_live;
   const int lane = Gr::lane();
-  float* s_dyn = reinterpret_cast<float*>(s_raw);
   using Rows = RowQueue<T, V, NV, G>;
   Rows rows(s_raw, logits, p.tokens, p.experts);
   rows.fill_rest(p.experts, lane);
   WordQueue<int> first_ids(s_raw + Rows::kBytes);
+  double* s_sums = reinterpret_cast<double*>(s_raw + Rows::kBytes + WordQueue<int>::kBytes);
   int* s_counts = reinterpret_cast<int*>(s_raw + p.counts_at);
   ptx::grid_wait();
   ptx::grid_launch_dependents();                           // the second kernel's blocks may take their places
@@ -101,6 +119,26 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+  double* part = p.part_p + static_cast<long long>(item) * p.width;
+  double* sums = G > 32 ? part : s_sums + Gr::index() * p.width;
+  bool begun = false;
+  auto flush = [&] {                                       // every thread its own columns: nobody to wait for
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int col = (i * G + lane) * V + j;
+        const double run = static_cast<double>(acc[i * V + j]);
+        if (col < p.width) {
+          if (!begun) sums[col] = run;
+          else if constexpr (G > 32) atomicAdd(&sums[col], run);       // (in global memory, and nothing to wait for)
+          else sums[col] += run;
+        }
+        acc[i * V + j] = 0.0f;
+      }
+    }
+    begun = true;
+  };
   int live_tokens = 0;
   int t = lo + Gr::index();                                // the next token to be worked on
   int ahead = t;                                           // ... to be fetched
@@ -130,6 +168,7 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
   const int steps = (hi - lo + Gr::kPerBlock - 1) / Gr::kPerBlock;
   for (int step = 0; step < steps; ++step) {
     const int stage = step & (kDepth - 1);
+    if (step != 0 && (step & (kRun - 1)) == 0) flush();
     fetch((step + kDepth - 1) & (kDepth - 1));
     queue_wait();
     float z[N];
@@ -175,21 +214,13 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
     }
   }
   if (lane == 0) atomicAdd(&s_live, live_tokens);
+  flush();
   asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();                                         // the queues become the rows of sums
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int col = (i * G + lane) * V + j;
-      if (col < p.width) s_dyn[Gr::index() * p.width + col] = acc[i * V + j];
-    }
-  }
-  __syncthreads();
+  __syncthreads();                                         // every group's sums, and the counts
   for (int e = threadIdx.x; e < p.width; e += kThreads) {
-    float sum = s_dyn[e];
-    for (int r = 1; r < Gr::kPerBlock; ++r) sum += s_dyn[r * p.width + e];
-    p.part_p[static_cast<long long>(item) * p.width + e] = sum;
+    if constexpr (G <= 32) {
+      part[e] = sum_rows<Gr::kPerBlock>([&](int r) { return s_sums[r * p.width + e]; });
+    }
     p.part_n[static_cast<long long>(item) * p.width + e] = s_counts[e];
   }
   if (threadIdx.x == 0) p.part_t[item] = make_int2(s, s_live);
@@ -203,7 +234,7 @@ balance_partial_kernel(const T* logits, const LossParams p) {
 }
 
 struct ReduceShared {
-  alignas(16) float p[16][64];             // (written four columns at a time)
+  alignas(16) double p[16][64];            // (written two and four columns at a time)
   alignas(16) int n[16][64];
   int tokens, count;
   double loss[kWarps];
@@ -227,19 +258,21 @@ __device__ __forceinline__ double reduce_columns(const LossParams& p, int s, int
   const int col = col_block * 64 + quad * 4;
   __syncthreads();
   partials_ready();
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  double2 sum = make_double2(0.0, 0.0), sum2 = sum;       // columns 0 and 1, 2 and 3
   int4 num = make_int4(0, 0, 0, 0);
   if (hi > lo && col < p.width) {
     const int first = lo / p.chunk + s, last = (hi - 1) / p.chunk + s;
 #pragma unroll 4
     for (int i = first + strand; i <= last; i += 16) {
-      const float4 a = *reinterpret_cast<const float4*>(p.part_p + static_cast<long long>(i) * p.width + col);
+      const double2* from = reinterpret_cast<const double2*>(p.part_p + static_cast<long long>(i) * p.width + col);
+      const double2 a = from[0], b = from[1];
       const int4 n = *reinterpret_cast<const int4*>(p.part_n + static_cast<long long>(i) * p.width + col);
-      sum.x += a.x; sum.y += a.y; sum.z += a.z; sum.w += a.w;
+      sum.x += a.x; sum.y += a.y; sum2.x += b.x; sum2.y += b.y;
       num.x += n.x; num.y += n.y; num.z += n.z; num.w += n.w;
     }
   }
-  *reinterpret_cast<float4*>(&sh.p[strand][quad * 4]) = sum;
+  *reinterpret_cast<double2*>(&sh.p[strand][quad * 4]) = sum;
+  *reinterpret_cast<double2*>(&sh.p[strand][quad * 4 + 2]) = sum2;
   *reinterpret_cast<int4*>(&sh.n[strand][quad * 4]) = num;
 #pragma unroll 2
   for (int i = threadIdx.x; i < items; i += kThreads) {
@@ -256,13 +289,10 @@ __device__ __forceinline__ double reduce_columns(const LossParams& p, int s, int
   __syncthreads();
   if (threadIdx.x < 64) {
     const int e = col_block * 64 + threadIdx.x;
-    float total = 0.0f;
+    const double total = sum_rows<16>([&](int r) { return sh.p[r][threadIdx.x]; });
     int n = 0;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      total += sh.p[r][threadIdx.x];
-      n += sh.n[r][threadIdx.x];
-    }
+    for (int r = 0; r < 16; ++r) n += sh.n[r][threadIdx.x];
     double term = 0.0;
     if (e < p.experts) {
       // alpha E n / (k T^2 S') in FP64, rounded once
@@ -384,7 +414,7 @@ LossLayout loss_layout(int tokens, int experts, int sequences) {
   const size_t rows = static_cast<size_t>(l.chunks) + sequences;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   l.p = 0;
-  l.n = up(l.p + rows * l.width * 4);
+  l.n = up(l.p + rows * l.width * 8);
   l.t = up(l.n + rows * l.width * 4);
   l.loss = up(l.t + rows * 8);
   l.ticket = up(l.loss + static_cast<size_t>(sequences) * l.col_blocks * 8);
@@ -400,14 +430,13 @@ struct LossLaunch {
     auto kernel = one ? balance_one_kernel<T, V, NV, G> : balance_partial_kernel<T, V, NV, G>;
     constexpr int kMaxWidth = G > 32 ? kMaxExperts : V * NV * G;
     constexpr size_t kQueues = RowQueue<T, V, NV, G>::kBytes + WordQueue<int>::kBytes;
-    constexpr size_t kSums = static_cast<size_t>(Group<G>::kPerBlock) * kMaxWidth * 4;
-    constexpr size_t kCountsAt = kQueues > kSums ? kQueues : kSums;
-    static_assert(kCountsAt % 16 == 0 && kCountsAt + kMaxWidth * 4 <= 112 * 1024, "two blocks per SM");
-    const int allowed = allow_smem(kernel, one ? once_one : once, one ? status_one : status, device,
-                                   static_cast<int>(kCountsAt + kMaxWidth * 4));
+    auto sums = [](int width) { return G > 32 ? 0 : static_cast<size_t>(Group<G>::kPerBlock) * width * 8; };
+    constexpr size_t kMost = kQueues + (G > 32 ? 0 : static_cast<size_t>(Group<G>::kPerBlock) * kMaxWidth * 8) + kMaxWidth * 4;
+    static_assert(kQueues % 16 == 0 && kMost <= 112 * 1024, "two blocks per SM");
+    const int allowed = allow_smem(kernel, one ? once_one : once, one ? status_one : status, device, static_cast<int>(kMost));
     if (allowed != B200_NVFP4_SUCCESS) return allowed;
-    p.counts_at = static_cast<int>(kCountsAt);
-    return launch_overlapped(kernel, one ? kOne : p.chunks + p.sequences, kThreads, kCountsAt + static_cast<size_t>(p.width) * 4, 1, stream,
+    p.counts_at = static_cast<int>(kQueues + sums(p.width));
+    return launch_overlapped(kernel, one ? kOne : p.chunks + p.sequences, kThreads, p.counts_at + static_cast<size_t>(p.width) * 4, 1, stream,
                              static_cast<const T*>(logits), p);
   }
 };
@@ -455,7 +484,7 @@ int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const voi
   p.width = l.width;
   p.alpha = alpha;
   p.softmax = scoring;
-  p.part_p = reinterpret_cast<float*>(ws + l.p);
+  p.part_p = reinterpret_cast<double*>(ws + l.p);
   p.part_n = reinterpret_cast<int*>(ws + l.n);
   p.part_t = reinterpret_cast<int2*>(ws + l.t);
   p.part_loss = reinterpret_cast<double*>(ws + l.loss);

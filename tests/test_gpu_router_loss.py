@@ -471,3 +471,19 @@ def test_around_what_one_launch_takes(ops, t, e, k, seqs):
     assert abs(float(loss) - float(wl)) <= float(wl) * (float(score_error(z).max()) * 2 + 96 * 2.0 ** -24)
     again = ops.router_balance_loss(z.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
     assert all(torch.equal(a, b) for a, b in zip((loss, counts, slope), again))
+
+
+@pytest.mark.parametrize("t,e", [(1 << 26, 7), (1 << 24, 13), (1 << 24, 100), (1 << 23, 200), (1 << 22, 520), (1 << 21, 1000), (1 << 20, 3000)])
+def test_sums_of_equal_probabilities_do_not_drift(ops, t, e):
+    """An indifferent router: every probability is 1 / E, whose roundings all go the same way, and the loss is 1 however
+    the slots fall. In units of 2^-24: a row's sum 20 additions of a thread, 5 and 8 of the group's; its reciprocal and the
+    quotient of the softmax 4 each at most; a run of 16 additions in FP32; the rest in FP64, the loss rounded once.
+    Nothing of it grows with the tokens."""
+    z = torch.full((t, e), 0.3, dtype=torch.bfloat16, device="cuda")
+    ids = (torch.arange(t, dtype=torch.int32, device="cuda") % e).view(t, 1)
+    for scoring in ("sigmoid", "softmax"):
+        loss, counts, slope = ops.router_balance_loss(z, ids, scoring=scoring)
+        assert abs(float(loss) - 1.0) <= (20 + 5 + 8 + 4 + 16 + 1) * 2.0 ** -24
+        want = torch.full((1, e), t // e, dtype=torch.int32, device="cuda")
+        want[0, :t % e] += 1
+        assert torch.equal(counts, want)
