@@ -41,7 +41,8 @@ struct LossParams {
   int* part_n;                // same
   int2* part_t;               // [chunks + sequences] (sequence, live tokens)
   double* part_loss;          // [sequences, column blocks]
-  unsigned* ticket;
+  unsigned* ticket;           // blocks of the last kernel that are done; beside it the sequences with a live token, where
+  int* live;                  // [sequences] the live tokens are counted first (nullptr: every block counts for itself)
   float* loss;
   int* counts;                // [S, E]
   float* slope;               // [S, E]
@@ -101,7 +102,7 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
   int* s_counts = reinterpret_cast<int*>(s_raw + p.counts_at);
   ptx::grid_wait();
   ptx::grid_launch_dependents();                           // the second kernel's blocks may take their places
-  if (item == 0 && threadIdx.x == 0) *p.ticket = 0;
+  if (item == 0 && threadIdx.x == 0) p.ticket[0] = p.ticket[1] = 0;
   const int s = item_sequence(p, item), c = item - s;
   int lo = 0, hi = 0;
   if (s < p.sequences && c < p.chunks) {
@@ -226,6 +227,28 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
   if (threadIdx.x == 0) p.part_t[item] = make_int2(s, s_live);
 }
 
+// Live tokens of every sequence and the number of sequences that have any, a warp per sequence. With few sequences
+// the blocks of the next kernel find both among all items themselves, which saves this launch; but that is sequences x
+// items in all. 65536 tokens x 256 in 32 / 128 / 256 / 512 / 1024 / 4096 / 16384 sequences, us with the scan: 23 / 31 / 38 / 50 /
+// 78 / 388 / 3842; with this kernel: 23 / 32 / 36 / 43 / 58 / 149 / 548. 4096 tokens x 64 in 128 / 256 / 512 / 1024: 8.3 / 9.0 /
+// 12.0 / 23 and 9.6 / 10.0 / 12.8 / 21.
+__global__ void __launch_bounds__(kThreads)
+balance_live_kernel(const LossParams p) {
+  const int s = static_cast<int>(blockIdx.x) * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int lo = s < p.sequences ? seq_start(p, s) : 0, hi = s < p.sequences ? seq_start(p, s + 1) : 0;
+  ptx::grid_wait();                                        // the items are complete
+  ptx::grid_launch_dependents();
+  int tokens = 0;
+  if (hi > lo) {
+    const int first = lo / p.chunk + s, last = (hi - 1) / p.chunk + s;
+    for (int i = first + lane; i <= last; i += 32) tokens += p.part_t[i].y;
+  }
+  tokens = __reduce_add_sync(0xffffffffu, tokens);
+  const int filled = __syncthreads_count(tokens > 0) / 32;
+  if (s < p.sequences && lane == 0) p.live[s] = tokens;
+  if (threadIdx.x == 0 && filled > 0) atomicAdd(&p.ticket[1], static_cast<unsigned>(filled));
+}
+
 template <typename T, int V, int NV, int G>
 __global__ void __launch_bounds__(kThreads, 2)
 balance_partial_kernel(const T* logits, const LossParams p) {
@@ -244,14 +267,15 @@ static_assert(alignof(ReduceShared) == 16, "rows of four");
 // Adds a sequence's partial rows for 64 columns (item order within sixteen interleaved strands, then the strands) and
 // writes counts and slopes; thread 0 gets their part of the loss. It is a chain of latencies, so everything
 // that does not depend on the partial sums happens before `partials_ready` waits for them, and independent
-// loads are issued together. `filled_bits`: one per sequence.
+// loads are issued together. `filled_bits`: one per sequence, where the live tokens have not been counted before.
 template <typename Ready>
 __device__ __forceinline__ double reduce_columns(const LossParams& p, int s, int col_block, unsigned* filled_bits, ReduceShared& sh,
                                                  Ready partials_ready) {
   const int items = p.chunks + p.sequences;
   const int words = (p.sequences + 31) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < words; i += kThreads) filled_bits[i] = 0;
+  const bool scan = p.live == nullptr;
+  for (int i = threadIdx.x; scan && i < words; i += kThreads) filled_bits[i] = 0;
   if (threadIdx.x == 0) { sh.tokens = 0; sh.count = 0; }
   const int lo = seq_start(p, s), hi = seq_start(p, s + 1);
   const int strand = threadIdx.x >> 4, quad = threadIdx.x & 15;
@@ -274,18 +298,23 @@ __device__ __forceinline__ double reduce_columns(const LossParams& p, int s, int
   *reinterpret_cast<double2*>(&sh.p[strand][quad * 4]) = sum;
   *reinterpret_cast<double2*>(&sh.p[strand][quad * 4 + 2]) = sum2;
   *reinterpret_cast<int4*>(&sh.n[strand][quad * 4]) = num;
+  if (scan) {
 #pragma unroll 2
-  for (int i = threadIdx.x; i < items; i += kThreads) {
-    const int2 t = p.part_t[i];
-    if (t.y > 0) {
-      atomicOr(&filled_bits[t.x >> 5], 1u << (t.x & 31));
-      if (t.x == s) atomicAdd(&sh.tokens, t.y);
+    for (int i = threadIdx.x; i < items; i += kThreads) {
+      const int2 t = p.part_t[i];
+      if (t.y > 0) {
+        atomicOr(&filled_bits[t.x >> 5], 1u << (t.x & 31));
+        if (t.x == s) atomicAdd(&sh.tokens, t.y);
+      }
     }
+    __syncthreads();
+    int filled = 0;
+    for (int i = threadIdx.x; i < words; i += kThreads) filled += __popc(filled_bits[i]);
+    if (filled) atomicAdd(&sh.count, filled);
+  } else if (threadIdx.x == 0) {
+    sh.tokens = p.live[s];
+    sh.count = static_cast<int>(p.ticket[1]);
   }
-  __syncthreads();
-  int filled = 0;
-  for (int i = threadIdx.x; i < words; i += kThreads) filled += __popc(filled_bits[i]);
-  if (filled) atomicAdd(&sh.count, filled);
   __syncthreads();
   if (threadIdx.x < 64) {
     const int e = col_block * 64 + threadIdx.x;
@@ -313,6 +342,7 @@ __device__ __forceinline__ double reduce_columns(const LossParams& p, int s, int
 // The loss from its parts, by one block, in a fixed order.
 __device__ __forceinline__ void sum_loss(const LossParams& p, long long terms, ReduceShared& sh) {
   double mine = 0.0;
+#pragma unroll 8
   for (long long i = threadIdx.x; i < terms; i += kThreads) mine += __ldcg(p.part_loss + i);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
@@ -327,7 +357,7 @@ __device__ __forceinline__ void sum_loss(const LossParams& p, long long terms, R
 }
 
 // One block per sequence and 64 columns; the last one to finish adds up the loss. Whatever ran before the first kernel
-// has ended when this one starts: that kernel lets it start only then.
+// has ended when this one (or the one between) starts: that kernel lets it start only then.
 __global__ void __launch_bounds__(kThreads)
 balance_reduce_kernel(const LossParams p) {
   extern __shared__ unsigned s_filled[];                   // one bit per sequence
@@ -396,8 +426,11 @@ int loss_chunk(int tokens, int experts, int sequences) {
 struct LossLayout {
   bool one;
   int chunk, chunks, width, col_blocks;
-  size_t p, n, t, loss, ticket, total;
+  size_t p, n, t, loss, ticket, live, total;
 };
+
+constexpr int kScanned = 256;  // sequences whose live tokens every block of the last kernel counts for itself
+
 
 LossLayout loss_layout(int tokens, int experts, int sequences) {
   LossLayout l;
@@ -418,7 +451,8 @@ LossLayout loss_layout(int tokens, int experts, int sequences) {
   l.t = up(l.n + rows * l.width * 4);
   l.loss = up(l.t + rows * 8);
   l.ticket = up(l.loss + static_cast<size_t>(sequences) * l.col_blocks * 8);
-  l.total = up(l.ticket + 4);
+  l.live = up(l.ticket + 8);
+  l.total = sequences > kScanned ? up(l.live + static_cast<size_t>(sequences) * 4) : l.live;
   return l;
 }
 
@@ -489,6 +523,7 @@ int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const voi
   p.part_t = reinterpret_cast<int2*>(ws + l.t);
   p.part_loss = reinterpret_cast<double*>(ws + l.loss);
   p.ticket = reinterpret_cast<unsigned*>(ws + l.ticket);
+  p.live = num_sequences > kScanned ? reinterpret_cast<int*>(ws + l.live) : nullptr;
   p.loss = static_cast<float*>(loss);
   p.counts = static_cast<int*>(counts);
   p.slope = static_cast<float*>(slope);
@@ -502,9 +537,13 @@ int b200_nvfp4_moe_balance_loss(void* loss, void* counts, void* slope, const voi
     default: status = dispatch_width<float, LossLaunch>(num_experts, quads, logits, p, l.one, dev.device, s); break;
   }
   if (status != B200_NVFP4_SUCCESS || l.one) return status;
-  // the second kernel may start while the first one drains: it waits for its end itself
-  return launch_overlapped(balance_reduce_kernel, dim3(num_sequences, l.col_blocks), kThreads, static_cast<size_t>((num_sequences + 31) / 32) * 4, 1,
-                           s, p);
+  // each of the next kernels may start while the one before drains: it waits for its end itself
+  if (num_sequences > kScanned) {
+    status = launch_overlapped(balance_live_kernel, (num_sequences + kWarps - 1) / kWarps, kThreads, 0, 1, s, p);
+    if (status != B200_NVFP4_SUCCESS) return status;
+  }
+  const size_t bits = num_sequences > kScanned ? 0 : static_cast<size_t>((num_sequences + 31) / 32) * 4;
+  return launch_overlapped(balance_reduce_kernel, dim3(num_sequences, l.col_blocks), kThreads, bits, 1, s, p);
 }
 
 }  // extern "C"

@@ -487,3 +487,72 @@ def test_sums_of_equal_probabilities_do_not_drift(ops, t, e):
         want = torch.full((1, e), t // e, dtype=torch.int32, device="cuda")
         want[0, :t % e] += 1
         assert torch.equal(counts, want)
+
+
+@pytest.mark.parametrize("t,e,k,seqs", [(900, 24, 3, 256), (900, 24, 3, 257), (2500, 40, 3, 3000), (700, 130, 4, 1500), (400, 600, 2, 500),
+                                        (1000, 5, 2, 65536)])
+def test_many_sequences(ops, t, e, k, seqs):
+    z, ids, cu, gw = case(t, e, k, seqs, t + seqs)
+    loss, counts, slope = ops.router_balance_loss(z.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
+    wl, wc, ws, live, seq = reference(z, ids, cu, "sigmoid", 1.0)
+    assert torch.equal(counts.cpu().long(), wc)
+    assert ((slope.cpu().double() - ws).abs() <= ws * 2.0 ** -23).all()
+    # positive terms: the score's error, and runs of 16 FP32 additions
+    assert abs(float(loss) - float(wl)) <= float(wl) * (float(score_error(z).max()) * 2 + 32 * 2.0 ** -24)
+    again = ops.router_balance_loss(z.cuda(), ids.cuda(), cu_seqlens=cu.cuda())
+    assert all(torch.equal(a, b) for a, b in zip((loss, counts, slope), again))
+    got = ops.router_backward(z.cuda(), ids.cuda(), slope=slope, grad_loss=torch.ones((), device="cuda"), cu_seqlens=cu.cuda())
+    want, size = reference_grad(z, ids, None, None, cu, ws, 1.0, "sigmoid", live, seq)
+    compare_grad(got, want, size, z)
+
+
+def test_time_grows_with_the_sequences_and_not_with_their_square(ops):
+    t, e = 65536, 64
+    z = torch.randn((t, e), device="cuda")
+    ids = z.topk(4).indices.to(torch.int32)
+
+    def time(seqs):
+        cu = torch.linspace(0, t, seqs + 1).to(torch.int32).cuda()
+        times = []
+        for _ in range(6):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            ops.router_balance_loss(z, ids, cu_seqlens=cu)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return sorted(times)[2]
+
+    few, many = time(4096), time(32768)
+    assert many < 24 * few, (few, many)        # eight times the sequences; their square would be 64
+
+
+def test_many_sequences_captured_and_written_right_before(ops):
+    t, e, k, seqs = 600, 32, 4, 700
+    cases = [case(t, e, k, seqs, i) for i in range(6)]
+    cases = [(z.cuda(), ids.cuda(), cu.cuda()) for z, ids, cu, _ in cases]
+    want = []
+    for z, ids, cu in cases:
+        want.append(ops.router_balance_loss(z, ids, cu_seqlens=cu))
+        torch.cuda.synchronize()
+    buffers = [torch.empty_like(x) for x in cases[0]]
+
+    def all_cases():
+        got = []
+        for c in cases:
+            for to, x in zip(buffers, c):
+                to.copy_(x)
+            got.append([x.clone() for x in ops.router_balance_loss(buffers[0], buffers[1], cu_seqlens=buffers[2])])
+        return got
+
+    for _ in range(10):
+        for a, w in zip(all_cases(), want):
+            assert all(torch.equal(x, y) for x, y in zip(a, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = all_cases()
+    for _ in range(10):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, w in zip(held, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, w))
