@@ -14,7 +14,7 @@
 //
 // Probabilities are added in FP32 for kRun tokens at most, then in FP64: equal ones (an indifferent router's) are
 // rounded the same way again and again, and one FP32 sum over n of them is off by up to n 2^-25 (2^22 tokens x 520: 1.7e-4,
-// 2^26 x 7: 8e-5; now below 3e-7 both). A run is off by 2^-21 at most, whatever the number of tokens. It costs nothing at
+// 2^26 x 7: 8e-5; now below 3e-7 both). A run is off by 2^-20 at most, whatever the number of tokens. It costs nothing at
 // 65536 x 256, 0.5 us at 4096 x 256 (8.5) and 3 % beyond 512 experts.
 //
 // 65536 x 256 FP32: 24.8 us where the bytes take 10.6; 131072 x 160 BF16: 25.6 us. In the first kernel no unit is
@@ -83,7 +83,10 @@ __device__ __forceinline__ double sum_rows(Value value) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-constexpr int kRun = 16;       // additions in FP32 before a sum goes into its FP64 one
+// Additions in FP32 before a sum goes into its FP64 one. (Twice as many where these are added to by atomic operations,
+// which are slow: 8192 x 4096 57 -> 53 us, 1048576 x 600 4767 -> 4699.)
+template <int G>
+constexpr int kRun = G > 32 ? 32 : 16;
 
 // Partial sums of one work item, written out. `s_raw`: queues, a row of sums per group, counts. (The one group of a
 // wide row adds up in its partial row itself: 32 KB of sums per block would leave room for one block per SM only.)
@@ -169,7 +172,7 @@ __device__ __forceinline__ void add_item(const T* logits, const LossParams& p, u
   const int steps = (hi - lo + Gr::kPerBlock - 1) / Gr::kPerBlock;
   for (int step = 0; step < steps; ++step) {
     const int stage = step & (kDepth - 1);
-    if (step != 0 && (step & (kRun - 1)) == 0) flush();
+    if (step != 0 && (step & (kRun<G> - 1)) == 0) flush();
     fetch((step + kDepth - 1) & (kDepth - 1));
     queue_wait();
     float z[N];
