@@ -910,7 +910,12 @@ class _BalanceLoss(torch.autograd.Function):
 class _TopkBalanced(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, num_topk, cu_seqlens, scoring, alpha):
-        ids, weights = router_topk(logits, num_topk)
+        t, e = logits.shape
+        if t:
+            ids, weights = router_topk(logits, num_topk)
+        else:
+            _check(0 < num_topk <= e <= 4096, "need 0 < num_topk <= num_experts <= 4096")
+            ids, weights = logits.new_empty((0, num_topk), dtype=torch.int32), logits.new_empty((0, num_topk))
         loss, counts, slope = _balance_forward(logits, ids, cu_seqlens, scoring, alpha)
         ctx.save_for_backward(logits, ids, weights, cu_seqlens, slope)
         ctx.scoring = scoring
@@ -956,6 +961,7 @@ def router_topk_balanced(logits: torch.Tensor, num_topk: int, *, cu_seqlens: Opt
     """router_topk for a router in training: FP32 logits [T, E] -> (topk_ids, topk_weights, loss, counts),
     ids and weights exactly router_topk's, loss and counts those of router_balance_loss. weights and loss
     are differentiable with respect to the logits; the backward pass is one kernel for both.
+    T may be 0, as on a rank without tokens: the loss is 0 then.
     """
     _check(logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32 and logits.is_contiguous(),
            "logits must be a contiguous float32 CUDA tensor [num_tokens, num_experts]")

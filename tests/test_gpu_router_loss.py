@@ -556,3 +556,18 @@ def test_many_sequences_captured_and_written_right_before(ops):
     torch.cuda.synchronize()
     for a, w in zip(held, want):
         assert all(torch.equal(x, y) for x, y in zip(a, w))
+
+
+@pytest.mark.parametrize("seqs", [0, 4])
+def test_balanced_router_without_tokens(ops, seqs):
+    # a rank that no token reaches takes part in the step all the same
+    leaf = torch.empty((0, 32), device="cuda", requires_grad=True)
+    cu = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda") if seqs else None
+    ids, weights, loss, counts = ops.router_topk_balanced(leaf, 4, cu_seqlens=cu, alpha=0.5)
+    assert ids.shape == (0, 4) and ids.dtype == torch.int32 and weights.shape == (0, 4) and weights.dtype == torch.float32
+    assert counts.shape == (max(seqs, 1), 32) and int(counts.abs().sum()) == 0 and float(loss.detach()) == 0
+    (loss + weights.sum()).backward()
+    assert leaf.grad.shape == (0, 32)
+    for k in (0, 33):
+        with pytest.raises(RuntimeError):
+            ops.router_topk_balanced(leaf, k)
