@@ -950,6 +950,8 @@ def router_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, *, cu_seql
     loss is differentiable with respect to the logits (counts are constants); slope is what
     router_backward needs to do the same by hand.
     """
+    if torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
+        _check(False, "router_balance_loss has no forward-mode derivative")
     if logits.requires_grad and torch.is_grad_enabled():
         return _BalanceLoss.apply(logits, topk_ids, cu_seqlens, scoring, alpha)
     return _balance_forward(logits, topk_ids, cu_seqlens, scoring, alpha)

@@ -571,3 +571,25 @@ def test_balanced_router_without_tokens(ops, seqs):
     for k in (0, 33):
         with pytest.raises(RuntimeError):
             ops.router_topk_balanced(leaf, k)
+
+
+def test_transformations_without_a_rule_are_refused(ops):
+    """Forward-mode derivatives and batched calls do not exist: they are refused, and nothing gets lost on the way."""
+    z, ids, _, _ = case(12, 16, 3, 0, 1, masked=0.0)
+    z, ids = z.cuda(), ids.cuda()
+    ahead = torch.autograd.forward_ad
+    loss = lambda x: ops.router_balance_loss(x, ids)[0]  # noqa: E731
+    step = lambda x: ops.router_topk_balanced(x, 3)[2]  # noqa: E731
+    for call in (loss, step):
+        with ahead.dual_level():
+            for x in (z, z.clone().requires_grad_()):
+                with pytest.raises(RuntimeError):
+                    call(ahead.make_dual(x, torch.ones_like(z)))
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call(ahead.make_dual(z, torch.ones_like(z)))
+            assert torch.isfinite(call(z))                              # an ordinary tensor beside dual ones
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (z,), (torch.ones_like(z),))
+        with pytest.raises(RuntimeError):
+            torch.vmap(call)(torch.stack((z, z)))
+    assert torch.isfinite(loss(z))
