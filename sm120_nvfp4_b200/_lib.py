@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib
+import warnings
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -104,15 +105,28 @@ def lib():
     return _lib
 
 
+class _NoCalls:
+    """Stands in for an extension module that cannot be had: declines every call, which then goes through ctypes."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def calls():
-    """The extension module that calls some entry points without ctypes (csrc/torch_calls.cpp)."""
+    """The extension module that calls some entry points without ctypes (csrc/torch_calls.cpp), built where it is
+    missing or was made from something else. Without a compiler for it, or where it does not load, the same
+    calls cost some microseconds more."""
     global _calls
     if _calls is None:
         lib()
         from . import build as _build
-        if not _build.CALLS.exists():
+        try:
             _build.build_calls()
-        _calls = importlib.import_module("._calls", __package__)
+            _calls = importlib.import_module("._calls", __package__)
+        except (RuntimeError, OSError, ImportError) as why:
+            warnings.warn(f"short calls go through ctypes, the extension module is not available: {why}", RuntimeWarning,
+                          stacklevel=2)
+            _calls = _NoCalls()
     return _calls
 
 

@@ -9,6 +9,7 @@ encode tensor maps is fetched at run time).
 """
 from __future__ import annotations
 
+import hashlib
 import os
 import subprocess
 import sys
@@ -27,6 +28,9 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
 
 
 CALLS = PKG / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+CALLS_MADE_FROM = PKG / "build" / "_calls.digest"
+_CALLS_SOURCE = CSRC / "torch_calls.cpp"
+_CALLS_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
 
 
 def _nvcc() -> str:
@@ -78,25 +82,43 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return OUT
 
 
+def _calls_digest() -> str:
+    """Of everything the extension module is made from: its source, the C ABI, torch, the interpreter, the flags."""
+    import torch
+    h = hashlib.sha256()
+    for part in (_CALLS_SOURCE.read_bytes(), (ROOT / "include" / "b200_nvfp4.h").read_bytes(), torch.__version__.encode(),
+                 sys.version.encode(), " ".join(_CALLS_FLAGS).encode()):
+        h.update(hashlib.sha256(part).digest())
+    return h.hexdigest()
+
+
 def build_calls(force: bool = False) -> Path:
     """The extension module of csrc/torch_calls.cpp: host code only, against the installed torch and this
-    package's library (found beside it at run time)."""
-    src = CSRC / "torch_calls.cpp"
-    if not (force or _stale(CALLS, [src, ROOT / "include" / "b200_nvfp4.h"])):
+    package's library (found beside it at run time). Built again where what it was made from has changed; several
+    processes may do so at once."""
+    made_from = CALLS_MADE_FROM.read_text() if CALLS_MADE_FROM.exists() else ""
+    digest = _calls_digest()
+    if CALLS.exists() and made_from == digest and not force:
         return CALLS
     import torch
     from torch.utils import cpp_extension
-    lib = build()
+    lib = OUT if OUT.exists() else build()
     includes = [*cpp_extension.include_paths(), os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include"),
                 sysconfig.get_path("include"), str(ROOT / "include")]
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes), str(src),
-           "-o", str(CALLS), f"-L{libs}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
-           f"-L{lib.parent}", f"-l:{lib.name}", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    made = CALLS.with_name(f"{CALLS.name}.{os.getpid()}")
+    cmd = ["g++", *_CALLS_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
+           str(_CALLS_SOURCE), "-o", str(made), f"-L{libs}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda",
+           "-lc10", f"-L{lib.parent}", f"-l:{lib.name}", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed for {_CALLS_SOURCE.name}:\n{res.stdout}\n{res.stderr}")
+        os.replace(made, CALLS)              # whole or not at all, for a process that loads it meanwhile
+    finally:
+        made.unlink(missing_ok=True)
+    CALLS_MADE_FROM.parent.mkdir(exist_ok=True)
+    CALLS_MADE_FROM.write_text(digest)
     return CALLS
 
 

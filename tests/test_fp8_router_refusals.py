@@ -190,3 +190,62 @@ def test_kernels_that_start_early_make_no_read_only_loads():
     for p in early + [p for p in sources if p.name == "router_common.cuh"]:
         code = re.sub(r"//[^\n]*", "", p.read_text())
         assert not re.search(r"__ldg|__restrict__|\.nc\b", code), p.name
+
+
+def test_calls_go_through_ctypes_where_the_extension_module_is_not_to_be_had(monkeypatch):
+    import importlib
+    import warnings
+    from sm120_nvfp4_b200 import _lib, build
+
+    def no_compiler(force=False):
+        raise FileNotFoundError("g++")
+
+    def no_module(name, package=None):
+        raise ImportError("undefined symbol")
+
+    for patch in ((build, "build_calls", no_compiler), (importlib, "import_module", no_module)):
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "_calls", None)
+            m.setattr(*patch)
+            with pytest.warns(RuntimeWarning, match="ctypes"):
+                declines = _lib.calls()
+            assert declines.fp8_gemm(1, 2, 3) is None and declines.balance_loss() is None
+            with warnings.catch_warnings():
+                warnings.simplefilter("error")
+                assert _lib.calls() is declines                            # said once
+    assert _lib.calls().__name__.endswith("_calls")
+
+
+def test_the_extension_module_is_built_again_when_its_source_changes(monkeypatch, tmp_path):
+    import os
+    import subprocess
+    from pathlib import Path
+    from sm120_nvfp4_b200 import build
+    source, runs = tmp_path / "torch_calls.cpp", []
+    source.write_text("one")
+
+    def compiler(cmd, **kwargs):
+        out = Path(cmd[cmd.index("-o") + 1])
+        assert out != build.CALLS and out.parent == build.CALLS.parent     # not into a file that somebody may be loading
+        out.write_text(source.read_text())
+        runs.append(out)
+        return subprocess.CompletedProcess(cmd, int("error" in source.read_text()), "", "")
+
+    monkeypatch.setattr(build, "CALLS", tmp_path / "_calls.so")
+    monkeypatch.setattr(build, "CALLS_MADE_FROM", tmp_path / "build" / "_calls.digest")
+    monkeypatch.setattr(build, "_CALLS_SOURCE", source)
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    assert build.build_calls().read_text() == "one" and len(runs) == 1
+    os.utime(source, (2 ** 31 - 10, 2 ** 31 - 10))                          # a copy of the tree has other dates
+    build.build_calls()
+    assert len(runs) == 1
+    source.write_text("two")
+    os.utime(source, (1, 1))
+    assert build.build_calls().read_text() == "two" and len(runs) == 2
+    source.write_text("error")
+    with pytest.raises(RuntimeError):
+        build.build_calls()
+    assert build.CALLS.read_text() == "two" and sorted(p.name for p in tmp_path.iterdir()) == ["_calls.so", "build", "torch_calls.cpp"]
+    build.CALLS.unlink()
+    source.write_text("two")
+    assert build.build_calls().read_text() == "two"
