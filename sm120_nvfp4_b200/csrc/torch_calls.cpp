@@ -66,6 +66,15 @@ PyObject* refuse(const char* what, int status) {
 
 void* stream_of(int index) { return at::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream(); }
 
+// The interpreter is free for other threads from here to the end of the scope: an allocation or a launch can wait for
+// the GPU (a launch does while the queue is full), and what the GPU waits for may be another thread's to do.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // A C++ exception (an allocation that failed) becomes the Python one torch has for it.
 template <typename Body>
 PyObject* guarded(Body body) {
@@ -111,11 +120,16 @@ PyObject* fp8_gemm(PyObject*, PyObject* const* args, Py_ssize_t count) {
     const int64_t m = a->size(0), k = a->size(1), n = b->size(0);
     if (!is_shape(sb, {blocks_128(n), blocks_128(k)})) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
-    const Tensor out = product_output(args[4], given, bad, m, n, index);
+    Tensor out;
+    int status = 0;
+    {
+      const Unlocked unlocked;
+      out = product_output(args[4], given, bad, m, n, index);
+      if (out.defined())
+        status = b200_nvfp4_fp8_gemm(static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), a->data_ptr(), b->data_ptr(),
+                                     sa->data_ptr(), sb->data_ptr(), out.data_ptr(), output_code(out.scalar_type()), stream_of(index));
+    }
     if (!out.defined()) Py_RETURN_NONE;
-    const int status = b200_nvfp4_fp8_gemm(static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), a->data_ptr(),
-                                           b->data_ptr(), sa->data_ptr(), sb->data_ptr(), out.data_ptr(),
-                                           output_code(out.scalar_type()), stream_of(index));
     if (status != 0) return refuse("b200_nvfp4_fp8_gemm", status);
     return THPVariable_Wrap(out);
   });
@@ -139,12 +153,17 @@ PyObject* fp8_grouped_gemm(PyObject*, PyObject* const* args, Py_ssize_t count) {
         seqlens->numel() != groups || cu->numel() != groups + 1)
       Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
-    const Tensor out = product_output(args[6], given, bad, m, n, index);
+    Tensor out;
+    int status = 0;
+    {
+      const Unlocked unlocked;
+      out = product_output(args[6], given, bad, m, n, index);
+      if (out.defined())
+        status = b200_nvfp4_fp8_grouped_gemm(out.data_ptr(), x->data_ptr(), w->data_ptr(), seqlens->data_ptr(), cu->data_ptr(),
+                                             xs->data_ptr(), ws->data_ptr(), static_cast<int>(groups), static_cast<int>(m),
+                                             static_cast<int>(n), static_cast<int>(k), 0, output_code(out.scalar_type()), stream_of(index));
+    }
     if (!out.defined()) Py_RETURN_NONE;
-    const int status = b200_nvfp4_fp8_grouped_gemm(out.data_ptr(), x->data_ptr(), w->data_ptr(), seqlens->data_ptr(),
-                                                   cu->data_ptr(), xs->data_ptr(), ws->data_ptr(), static_cast<int>(groups),
-                                                   static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), 0,
-                                                   output_code(out.scalar_type()), stream_of(index));
     if (status != 0) return refuse("b200_nvfp4_fp8_grouped_gemm", status);
     return THPVariable_Wrap(out);
   });
@@ -169,10 +188,15 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t count) {
         (!on(given_scale, index) || given_scale->scalar_type() != ScalarType::Float || !is_shape(given_scale, {rows, kb})))
       Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
-    const Tensor q = given != nullptr ? *given : empty({rows, k}, ScalarType::Float8_e4m3fn, index);
-    const Tensor s = given_scale != nullptr ? *given_scale : empty({rows, kb}, ScalarType::Float, index);
-    const int status = b200_nvfp4_fp8_quantize_rows(q.data_ptr(), s.data_ptr(), x->data_ptr(), static_cast<int>(rows),
-                                                    static_cast<int>(k), code, swiglu, stream_of(index));
+    Tensor q, s;
+    int status = 0;
+    {
+      const Unlocked unlocked;
+      q = given != nullptr ? *given : empty({rows, k}, ScalarType::Float8_e4m3fn, index);
+      s = given_scale != nullptr ? *given_scale : empty({rows, kb}, ScalarType::Float, index);
+      status = b200_nvfp4_fp8_quantize_rows(q.data_ptr(), s.data_ptr(), x->data_ptr(), static_cast<int>(rows), static_cast<int>(k),
+                                            code, swiglu, stream_of(index));
+    }
     if (status != 0) return refuse("b200_nvfp4_fp8_quantize_rows", status);
     return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s));
   });
@@ -219,15 +243,20 @@ PyObject* balance_loss(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (PyErr_Occurred()) return nullptr;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(r.index));
     const int tokens = static_cast<int>(r.tokens), experts = static_cast<int>(r.experts), sequences = static_cast<int>(r.sequences);
-    const size_t need = b200_nvfp4_moe_balance_loss_workspace_bytes(tokens, experts, sequences);
-    const Tensor loss = empty({}, ScalarType::Float, r.index);
-    const Tensor counts = empty({r.sequences, r.experts}, ScalarType::Int, r.index);
-    const Tensor slope = empty({r.sequences, r.experts}, ScalarType::Float, r.index);
-    const Tensor workspace = empty({static_cast<int64_t>(need)}, ScalarType::Byte, r.index);
-    const int status = b200_nvfp4_moe_balance_loss(loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), r.logits->data_ptr(),
-                                                   r.ids->data_ptr(), data_or_null(r.cu), tokens, experts, static_cast<int>(r.topk),
-                                                   sequences, r.code, static_cast<int>(scoring), static_cast<float>(alpha),
-                                                   workspace.data_ptr(), need, stream_of(r.index));
+    Tensor loss, counts, slope;
+    int status = 0;
+    {
+      const Unlocked unlocked;
+      const size_t need = b200_nvfp4_moe_balance_loss_workspace_bytes(tokens, experts, sequences);
+      loss = empty({}, ScalarType::Float, r.index);
+      counts = empty({r.sequences, r.experts}, ScalarType::Int, r.index);
+      slope = empty({r.sequences, r.experts}, ScalarType::Float, r.index);
+      const Tensor workspace = empty({static_cast<int64_t>(need)}, ScalarType::Byte, r.index);
+      status = b200_nvfp4_moe_balance_loss(loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), r.logits->data_ptr(), r.ids->data_ptr(),
+                                           data_or_null(r.cu), tokens, experts, static_cast<int>(r.topk), sequences, r.code,
+                                           static_cast<int>(scoring), static_cast<float>(alpha), workspace.data_ptr(), need,
+                                           stream_of(r.index));
+    }
     if (status != 0) return refuse("b200_nvfp4_moe_balance_loss", status);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(loss), THPVariable_Wrap(counts), THPVariable_Wrap(slope));
   });
@@ -254,12 +283,17 @@ PyObject* router_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
          grad_loss->scalar_type() != ScalarType::Float || grad_loss->numel() != 1))
       Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(r.index));
-    const Tensor grad = empty({r.tokens, r.experts}, r.logits->scalar_type(), r.index);
-    const int status = b200_nvfp4_moe_router_backward(
-        grad.data_ptr(), r.logits->data_ptr(), r.ids->data_ptr(), grad_weights != nullptr ? weights->data_ptr() : nullptr,
-        data_or_null(grad_weights), data_or_null(slope), slope != nullptr ? grad_loss->data_ptr() : nullptr, data_or_null(r.cu),
-        static_cast<int>(r.tokens), static_cast<int>(r.experts), static_cast<int>(r.topk), static_cast<int>(r.sequences), r.code,
-        static_cast<int>(scoring), stream_of(r.index));
+    Tensor grad;
+    int status = 0;
+    {
+      const Unlocked unlocked;
+      grad = empty({r.tokens, r.experts}, r.logits->scalar_type(), r.index);
+      status = b200_nvfp4_moe_router_backward(
+          grad.data_ptr(), r.logits->data_ptr(), r.ids->data_ptr(), grad_weights != nullptr ? weights->data_ptr() : nullptr,
+          data_or_null(grad_weights), data_or_null(slope), slope != nullptr ? grad_loss->data_ptr() : nullptr, data_or_null(r.cu),
+          static_cast<int>(r.tokens), static_cast<int>(r.experts), static_cast<int>(r.topk), static_cast<int>(r.sequences), r.code,
+          static_cast<int>(scoring), stream_of(r.index));
+    }
     if (status != 0) return refuse("b200_nvfp4_moe_router_backward", status);
     return THPVariable_Wrap(grad);
   });

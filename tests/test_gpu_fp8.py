@@ -721,3 +721,44 @@ def test_silu_does_not_depend_on_the_values_beside_it(ops, dtype):
         v = gates.double() / (1.0 + torch.exp(-gates.double())) * up
         want = v.abs().clamp(min=2.0 ** -60) / 448.0
         assert ((s[:, 0].cpu().double() - want).abs() <= 8 * 2.0 ** -24 * want).all()
+
+
+def test_other_threads_run_while_a_launch_waits(ops):
+    # behind a busy GPU the queue of launches fills up; whoever launches then waits, and must not hold up the other threads
+    import threading
+    import time
+    a, sa = codes(4, 256, 1)
+    b, sb = weight(64, 256, 2)
+    x = torch.randn((4, 256), device="cuda")
+    z = torch.randn((8, 16), device="cuda")
+    ids = z.topk(2).indices.to(torch.int32)
+    slope, one = torch.zeros((1, 16), device="cuda"), torch.ones((), device="cuda")
+    w, sw = b.view(torch.uint8).view(1, 64, 256).view(E4M3), sb.view(1, *sb.shape)
+    n1, cu = torch.tensor([4], dtype=torch.int32, device="cuda"), torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    calls = [lambda: ops.fp8_gemm(a, b, sa, sb), lambda: ops.fp8_grouped_gemm(a, w, n1, cu, sa, sw), lambda: ops.quantize_fp8(x),
+             lambda: ops.router_balance_loss(z, ids), lambda: ops.router_backward(z, ids, slope=slope, grad_loss=one)]
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        done = threading.Event()
+
+        def launch():
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(800_000_000)            # some 0.4 s
+                for _ in range(2000):
+                    call()
+            done.set()
+
+        worker = threading.Thread(target=launch)
+        began = last = time.perf_counter()
+        worst = 0.0
+        worker.start()
+        while not done.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            worst, last = max(worst, now - last), now
+        worker.join()
+        torch.cuda.synchronize()
+        assert last - began > 0.25, "the queue did not fill up"
+        assert worst < 0.1, worst
