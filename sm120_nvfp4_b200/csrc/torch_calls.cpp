@@ -23,7 +23,7 @@ namespace {
 using at::ScalarType;
 using at::Tensor;
 
-constexpr int64_t kMost = 0x7fffff00, kMostTokens = 1 << 30;
+constexpr int64_t kMost = 0x7fffff00, kMostTokens = 1 << 30, kMostGroups = 1024;
 
 int64_t blocks_128(int64_t n) { return (n + 127) / 128; }
 
@@ -149,7 +149,7 @@ PyObject* fp8_grouped_gemm(PyObject*, PyObject* const* args, Py_ssize_t count) {
         seqlens->scalar_type() != ScalarType::Int || cu->scalar_type() != ScalarType::Int)
       Py_RETURN_NONE;
     const int64_t groups = w->size(0), m = x->size(0), k = x->size(1), n = w->size(1);
-    if (groups <= 0 || groups > 256 || groups * n > kMost || !is_shape(ws, {groups, blocks_128(n), blocks_128(k)}) ||
+    if (groups <= 0 || groups > kMostGroups || groups * n > kMost || !is_shape(ws, {groups, blocks_128(n), blocks_128(k)}) ||
         seqlens->numel() != groups || cu->numel() != groups + 1)
       Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));

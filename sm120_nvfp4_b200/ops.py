@@ -769,7 +769,7 @@ def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tenso
     [rows, K] times weight[g] ([groups, N, K]) transposed; x_scale [rows, ceil(K/128)], weight_scale
     [groups, ceil(N/128), ceil(K/128)]. seqlens int32 [groups] and cu_seqlens int32 [groups + 1] stay on
     the device; the ranges must not overlap. Rows that belong to no group keep what `output` held (without
-    `output` they are undefined). groups <= 256; otherwise as fp8_gemm.
+    `output` they are undefined). groups <= 1024; otherwise as fp8_gemm.
     """
     done = _lib.calls().fp8_grouped_gemm(x, weight, seqlens, cu_seqlens, x_scale, weight_scale, out_dtype, output)
     if done is not None:
@@ -783,8 +783,8 @@ def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tenso
     index, rows, n, k, out = _fp8_operands(x, weight, x_scale, weight_scale, out_dtype, output,
                                            ("x", "weight", "x_scale", "weight_scale"))
     groups = weight.shape[0]
-    if not (0 < groups <= 256):
-        _check(False, "number of groups must be in [1, 256]")
+    if not (0 < groups <= 1024):
+        _check(False, "number of groups must be in [1, 1024]")
     _on_device(index, (seqlens, cu_seqlens), ("seqlens", "cu_seqlens"))
     if not (seqlens.dtype == torch.int32 and cu_seqlens.dtype == torch.int32):
         _check(False, "seqlens and cu_seqlens must be int32")

@@ -762,3 +762,27 @@ def test_other_threads_run_while_a_launch_waits(ops):
         torch.cuda.synchronize()
         assert last - began > 0.25, "the queue did not fill up"
         assert worst < 0.1, worst
+
+
+@pytest.mark.parametrize("groups", [257, 1024])
+@pytest.mark.parametrize("most,tile", [(3, 0), (3, 64), (40, 0), (40, 128), (40, 512)])
+def test_grouped_product_of_as_many_groups_as_the_c_entry_takes(ops, L, groups, most, tile):
+    rng = np.random.default_rng(groups + most)
+    counts = rng.integers(0, most + 1, groups).astype(np.int32)
+    counts[-1] = most
+    cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    rows, n, k = int(cu[-1]), 264, 144
+    x, sx = codes(rows, k, 1)
+    g = torch.Generator().manual_seed(5)
+    w = (torch.randn((groups, n, k), generator=g) * 8).to(E4M3).cuda()
+    sw = torch.rand((groups, blocks(n), blocks(k)), generator=g).cuda()
+    assert L.b200_nvfp4_fp8_set_tile(tile, 0) == 0
+    args = (x, w, torch.from_numpy(counts).cuda(), torch.from_numpy(cu).cuda(), sx, sw)
+    out = ops.fp8_grouped_gemm(*args, out_dtype=torch.float32)
+    for e in range(groups):
+        lo, hi = cu[e], cu[e + 1]
+        if hi > lo:
+            want, total = reference(x[lo:hi], sx[lo:hi], w[e], sw[e])
+            check(out[lo:hi], want, total, k)
+    with pytest.raises(RuntimeError):
+        ops.fp8_grouped_gemm(x, w.new_empty((1025, 8, 16)), args[2], args[3], sx, sw)
