@@ -464,7 +464,10 @@ struct LossLaunch {
   static int run(const void* logits, LossParams p, bool one, int device, cudaStream_t stream) {
     static std::once_flag once[64], once_one[64];
     static cudaError_t status[64], status_one[64];
-    auto kernel = one ? balance_one_kernel<T, V, NV, G> : balance_partial_kernel<T, V, NV, G>;
+    auto kernel = balance_partial_kernel<T, V, NV, G>;
+    if constexpr (G <= 32) {                               // (more than 512 experts never go through one launch)
+      if (one) kernel = balance_one_kernel<T, V, NV, G>;
+    }
     constexpr int kMaxWidth = G > 32 ? kMaxExperts : V * NV * G;
     constexpr size_t kQueues = RowQueue<T, V, NV, G>::kBytes + WordQueue<int>::kBytes;
     auto sums = [](int width) { return G > 32 ? 0 : static_cast<size_t>(Group<G>::kPerBlock) * width * 8; };
