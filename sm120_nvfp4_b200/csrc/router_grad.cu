@@ -60,12 +60,14 @@ router_grad_kernel(T* grad, const T* logits, const GradParams p) {
   int t = begin + Gr::in_warp();
   // sequence of the first token: the number of sequence ends at or before it
   int s = 0, s_begin = 0, s_end = p.tokens;
-  if (p.cu && through_loss) {
-    int hi = p.sequences;
+  auto search = [&](int hi) {
     while (s < hi) {
       const int mid = (s + hi) >> 1;
       if (p.cu[mid + 1] <= t) s = mid + 1; else hi = mid;
     }
+  };
+  if (p.cu && through_loss) {
+    search(p.sequences);
     s_begin = s < p.sequences ? p.cu[s] : p.tokens;
     s_end = s < p.sequences ? p.cu[s + 1] : 0x7fffffff;
   }
@@ -130,7 +132,9 @@ router_grad_kernel(T* grad, const T* logits, const GradParams p) {
       }
     }
     if (t >= s_end && in) {                                // on to the sequence of this token
-      while (s < p.sequences && p.cu[s + 1] <= t) ++s;
+      // mostly the next one; behind padding of empty sequences, far on
+      for (int i = 0; i < 4 && s < p.sequences && p.cu[s + 1] <= t; ++i) ++s;
+      if (s < p.sequences && p.cu[s + 1] <= t) search(p.sequences);
       s_begin = s < p.sequences ? p.cu[s] : p.tokens;
       s_end = s < p.sequences ? p.cu[s + 1] : 0x7fffffff;
       load_slope();

@@ -593,3 +593,36 @@ def test_transformations_without_a_rule_are_refused(ops):
         with pytest.raises(RuntimeError):
             torch.vmap(call)(torch.stack((z, z)))
     assert torch.isfinite(loss(z))
+
+
+def test_padding_of_empty_sequences(ops):
+    """cu_seqlens of a fixed length, its rest filled with the end of the last sequence and tokens behind that: same results, and
+    nobody walks through the empty sequences one by one (of 65536, that took five hundred times as long as the kernel)."""
+    t, e, k, used = 20000, 64, 4, 30
+    z, ids, _, gw = case(t, e, k, 0, 9)
+    z, ids = z.cuda(), ids.cuda()
+    ends = torch.linspace(0, t - 37, used + 1).to(torch.int32)
+    one = torch.ones((), device="cuda")
+    results, times = [], []
+    for seqs in (used, 65536):
+        cu = torch.cat([ends[:12], ends[11].repeat((seqs - used) // 2), ends[12:], ends[-1].repeat(seqs - used - (seqs - used) // 2)]).cuda()
+        assert cu.numel() == seqs + 1
+        loss, counts, slope = ops.router_balance_loss(z, ids, cu_seqlens=cu)
+        grad = ops.router_backward(z, ids, slope=slope, grad_loss=one, cu_seqlens=cu)
+        results.append((loss, counts[counts.sum(1) > 0], slope[slope.sum(1) > 0], grad))
+        spent = []
+        for _ in range(7):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            begin.record()
+            for _ in range(10):
+                ops.router_backward(z, ids, slope=slope, grad_loss=one, cu_seqlens=cu)
+            end.record()
+            torch.cuda.synchronize()
+            spent.append(begin.elapsed_time(end))
+        times.append(sorted(spent)[3])
+    # chunks of tokens, and with them the order of the sums, go by the number of sequences: at most a unit of the loss
+    assert abs(float(results[0][0]) - float(results[1][0])) <= 2.0 ** -23 * float(results[0][0])
+    assert torch.equal(results[0][1], results[1][1]) and torch.equal(results[0][2], results[1][2])
+    assert torch.equal(results[0][3], results[1][3])
+    assert times[1] < 4 * times[0], times
