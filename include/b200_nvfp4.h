@@ -505,8 +505,8 @@ B200_NVFP4_API int b200_nvfp4_fp8_set_tile(int tile, int splits);
 
 /* Rows to E4M3 with one FP32 scale per 128 values of K: amax = max |x| over the block (at least 2^-60),
  * scale = RN(amax / 448), q = E4M3(RN(x / scale)). x [rows, K] row-major of input_dtype 0 = FP16, 1 = BF16,
- * 2 = FP32; with swiglu != 0 x is [rows, 2K], gate then up, and silu(gate) * up (each
- * step rounded to FP32) is quantised. q [rows, K] bytes, scale [rows,
+ * 2 = FP32; with swiglu != 0 x is [rows, 2K], gate then up, and silu(gate) * up =
+ * gate / (1 + expf(-gate)) * up, each step rounded to FP32, is quantised: the same bits in any batch. q [rows, K] bytes, scale [rows,
  * ceil(K/128)]; x and q 16-byte aligned, K % 16 == 0, rows >= 0, less than
  * 2^31 blocks. A block that holds a NaN or an
  * infinity gets a NaN or infinite scale. What b200_nvfp4_fp8_gemm takes as A and a_scale. */

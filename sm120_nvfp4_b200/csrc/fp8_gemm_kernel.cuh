@@ -24,9 +24,9 @@
 //                          kWide = true: 128 rows of A on the 128-row side, one scale per thread.
 //   fp8_pair_kernel        many rows: 256 x 256 tiles on CTA pairs (cta_group::2).
 //
-// What bounds them, measured back to back with cold operands. One row, 4096 x 7168: 7.6 us for 29.4 MB, of which HBM
+// What bounds them, measured back to back with cold operands. One row, 4096 x 7168: 7.5 us for 29.4 MB, of which HBM
 // takes 4.5; the rest is the first loads' latency, the exchange of partial tiles and the stores. 77 x 1000 x
-// 1040: 5.2 us of fixed costs and dependent blocks, as short as Python can issue them. 128 x 4096 x 8192: 14.5 us;
+// 1040: 5.2 us of fixed costs and dependent blocks, as short as Python can issue them. 128 x 4096 x 8192: 14.0 us;
 // 16 blocks per CTA at 0.335 us, which is 128 SMs taking 32 KB each from L2 (12.5 TB/s), and the exchange.
 // 64 rows over 32 groups of 4096 x 7168: 125 us, HBM (765 MB, 6.1 TB/s; weights of empty groups are not
 // read). Many rows: see the pair kernel.
@@ -610,7 +610,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 // promotion warps need more registers than an even share (65536 / 384 = 168): the other four warps
 // give theirs up (104 + 2 x 200 = 504 = 3 x 168; 56 / 224 to 104 / 200 differ by what the compiler spills: measured).
 //
-// 8192^3: 479 us in a burst (2300 TFLOP/s), 558 us sustained (1970 TFLOP/s, 0.71 of twice the measured BF16 rate),
+// 8192^3: 479 us in a burst (2300 TFLOP/s), 561 us sustained (1960 TFLOP/s, 0.71 of twice the measured BF16 rate),
 // where power holds the SM clock at 1.46 GHz. The same loads and MMAs with nothing done to their sums take
 // 394 / 466 us, bound by the operands' way from L2 (13.7 TB/s); promotion adds one TMEM read and one FMA per
 // value and block. 4096 x 4096 x 7168 under counters: tensor pipe 60 % of the cycles, FMA pipe 35 %, issue

@@ -5,7 +5,8 @@
 //
 // Reads 2 bytes (4 with SiLU) and writes 1.03 per value of a 16-bit input. Eight (or sixteen) lanes share a
 // block: 16-byte loads, an amax by three (four) exchanges, one 16-byte (8-byte) store. 32768 x 4096 BF16:
-// 69 us, 0.90 of what the bytes take at the measured copy rate. 32768 x 2048 with SiLU: 65.5 us, 0.79 of it: 25
+// 69 us, 0.90 of what the bytes take at the measured copy rate. 32768 x 2048 with SiLU: 66 to 69 us in bursts of some
+// hundred calls, 0.75 to 0.78 of it, and 73 to 77, 0.67 to 0.70, in runs of a second: 25
 // instructions per value, half of them the exponential and the division of the SiLU, at 76 % of the issue
 // slots, and the wait for the loads. (Both 2 us more without the overlapped start.)
 //

@@ -17,9 +17,9 @@
 // 2^26 x 7: 8e-5; now below 3e-7 both). A run is off by 2^-20 at most, whatever the number of tokens. It costs nothing at
 // 65536 x 256, 0.5 us at 4096 x 256 (8.5) and 3 % beyond 512 experts.
 //
-// 65536 x 256 FP32: 24.8 us where the bytes take 10.6; 131072 x 160 BF16: 25.6 us. In the first kernel no unit is
+// 65536 x 256 FP32: 24.6 us where the bytes take 10.6 (softmax 23.7); 131072 x 160 BF16: 26.0 us (23.5). In the first kernel no unit is
 // full: the special-function unit is busy for 7.4 us (an exponential and a reciprocal per logit, sixteen a
-// cycle per SM), 44 % of the issue slots are used; with 16 warps per SM the rest is the latency of dependent
+// cycle per SM), 45 % of the issue slots are used; with 16 warps per SM the rest is the latency of dependent
 // instructions, and that of the start and the end of blocks with 14 rounds of tokens each. The second
 // kernel is a chain of latencies, 7 us on its own, of which its early start hides a part.
 #include "router_common.cuh"
@@ -439,7 +439,7 @@ LossLayout loss_layout(int tokens, int experts, int sequences) {
   LossLayout l;
   // A call for a few tokens is launches more than anything: where the kOne blocks of a cluster, less one for each
   // sequence's end, get through the tokens in four steps each, and through the sums in one, one launch does
-  // it all (120 x 64, 3 sequences: 7.6 -> 6.1 us, and 8.7 -> 6.2 on the host; with two rounds of sums
+  // it all (64 x 64: 7.4 -> 6.5 us, 120 x 64 in 3 sequences 6.5 -> 6.2, and 8.4 -> 6.5 on the host; with two rounds of sums
   // 300 x 160, 3 sequences, took 8.6 against 7.5).
   const int most = experts <= 256 ? 64 : 32;
   l.one = sequences < kOne && sequences * ((experts + 63) / 64) <= kOne && tokens <= most * (kOne - sequences);

@@ -801,6 +801,7 @@ def fp8_grouped_gemm(x: torch.Tensor, weight: torch.Tensor, seqlens: torch.Tenso
 # Training side of the router step: balance loss, per-expert counts and the gradient of the logits.
 
 _SCORING = {"sigmoid": 0, "softmax": 1}
+_forward_ad = torch.autograd.forward_ad      # (its level first: unpack_dual alone costs half a microsecond)
 
 
 def _check_router(logits, topk_ids, cu_seqlens, scoring):
@@ -950,7 +951,7 @@ def router_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, *, cu_seql
     loss is differentiable with respect to the logits (counts are constants); slope is what
     router_backward needs to do the same by hand.
     """
-    if torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(logits).tangent is not None:
         _check(False, "router_balance_loss has no forward-mode derivative")
     if logits.requires_grad and torch.is_grad_enabled():
         return _BalanceLoss.apply(logits, topk_ids, cu_seqlens, scoring, alpha)
