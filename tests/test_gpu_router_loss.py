@@ -478,7 +478,8 @@ def test_sums_of_equal_probabilities_do_not_drift(ops, t, e):
     """An indifferent router: every probability is 1 / E, whose roundings all go the same way, and the loss is 1 however
     the slots fall. In units of 2^-24: a row's sum 20 additions of a thread, 5 and 8 of the group's; its reciprocal and the
     quotient of the softmax 4 each at most; a run of 16 additions in FP32; the rest in FP64, the loss rounded once.
-    Nothing of it grows with the tokens."""
+    (Beyond 512 experts a thread has 16 columns and a run 32 additions, the i-th of them off by i / 32 of the run's last
+    unit: 16.5 in all.) Nothing of it grows with the tokens."""
     z = torch.full((t, e), 0.3, dtype=torch.bfloat16, device="cuda")
     ids = (torch.arange(t, dtype=torch.int32, device="cuda") % e).view(t, 1)
     for scoring in ("sigmoid", "softmax"):
